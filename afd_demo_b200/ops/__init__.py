@@ -24,7 +24,8 @@ _KERNEL_CALLS = {"gemm", "sum_rmsnorm", "qk_norm_rope_cache", "decode_attention"
                  "prefill_attention", "router_topk", "moe_align", "moe_gather", "moe_combine",
                  "argmax", "signal_flags", "wait_flags", "add_i32", "peer_copy",
                  "decode_attention_fused", "moe_route", "moe_gate", "gemm_down_combine",
-                 "moe_align_mt", "decode_attention_tc"}
+                 "moe_align_mt", "decode_attention_tc", "paged_decode_attention",
+                 "packed_attention", "paged_prefill_attention", "norm_rope", "token_logprobs"}
 
 
 class LaunchCounter:
@@ -923,3 +924,9 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
 
 def rope_table(max_pos: int, head_dim: int, theta: float, device) -> torch.Tensor:
     return torch_ref.rope_table(max_pos, head_dim, theta, device, torch.bfloat16)
+
+
+# ---------------------------------------------- ragged batches, paged cache --
+from .ragged import (TokenLogprobs, packed_attention, paged_decode_attention,  # noqa: E402
+                     paged_prefill_attention, qk_norm_rope_packed, qk_norm_rope_paged,
+                     token_logprobs)

@@ -199,3 +199,153 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
 
 def stack_parts(parts: List[torch.Tensor]) -> torch.Tensor:
     return torch.stack(parts, 0)
+
+
+# ---------------------------------------------- ragged batches, paged cache --
+def _check(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _check_heads(nq: int, nkv: int) -> None:
+    _check(nkv >= 1 and nq >= 1 and nq % nkv == 0,
+           f"query heads ({nq}) must be a multiple of the kv heads ({nkv})")
+
+
+def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, D: int) -> None:
+    _check(k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
+           "k_pages and v_pages must be [pages, kv heads, page_size, head_dim], laid out alike")
+    _check(k_pages.shape[3] == D, "q and the pages differ in head_dim")
+    _check(k_pages.shape[2] >= 16 and k_pages.shape[2] % 16 == 0,
+           "page_size must be a multiple of 16, at most 4096")
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                 rope: torch.Tensor, positions: torch.Tensor, nq: int, nkv: int, eps: float
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMSNorm and RoPE in fp32 with one rounding: (q, k)."""
+    D = q_norm.shape[0]
+    T = qkv.shape[0]
+    _check_heads(nq, nkv)
+    _check(qkv.dim() == 2 and qkv.shape[1] == (nq + 2 * nkv) * D,
+           f"qkv must be [tokens, {(nq + 2 * nkv) * D}]")
+    _check(positions.dtype == torch.int32 and positions.numel() == T,
+           f"positions must be a contiguous int32 tensor of {T} on the same device")
+    x = qkv[:, : (nq + nkv) * D].reshape(T, nq + nkv, D).float()
+    w = torch.cat([q_norm.expand(nq, D), k_norm.expand(nkv, D)]).float()
+    x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w
+    cs = rope[positions.long()][:, None]
+    cos, sin = cs[..., : D // 2], cs[..., D // 2:]
+    lo, hi = x[..., : D // 2], x[..., D // 2:]
+    x = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], -1).to(qkv.dtype)
+    return x[:, :nq].contiguous(), x[:, nq:].contiguous()
+
+
+def qk_norm_rope_paged(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                       rope: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                       positions: torch.Tensor, slots: torch.Tensor, nq: int, nkv: int,
+                       eps: float) -> torch.Tensor:
+    """``qk_norm_rope`` with k and v stored at the page rows `slots` (negative:
+    not stored). Returns q."""
+    D, T = q_norm.shape[0], qkv.shape[0]
+    _check_pool(k_pages, v_pages, D)
+    _check(slots.dtype == torch.int64 and slots.numel() == T,
+           "slots must be a contiguous int64 tensor, one per token")
+    q, k = qk_norm_rope(qkv, q_norm, k_norm, rope, positions, nq, nkv, eps)
+    at = slots >= 0
+    page, row = slots[at] // k_pages.shape[2], slots[at] % k_pages.shape[2]
+    k_pages[page, :, row] = k[at]
+    v_pages[page, :, row] = qkv[:, (nq + nkv) * D:].reshape(T, nkv, D)[at]
+    return q
+
+
+def _causal_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float]
+                 ) -> torch.Tensor:
+    """q [n, nq, D] as the last n of the m positions of k, v [m, nkv, D]; a
+    query before the first key gives zeros. [n, nq * D]."""
+    n, nq, D = q.shape
+    m, nkv, _ = k.shape
+    kf = k.float().repeat_interleave(nq // nkv, 1)
+    vf = v.float().repeat_interleave(nq // nkv, 1)
+    s = torch.einsum("nhd,mhd->hnm", q.float(), kf) * (D ** -0.5 if scale is None else scale)
+    pos = m - n + torch.arange(n, device=q.device)
+    s = s.masked_fill(torch.arange(m, device=q.device)[None] > pos[:, None], float("-inf"))
+    p = torch.softmax(s, -1).masked_fill((pos < 0)[None, :, None], 0.0)
+    return torch.einsum("hnm,mhd->nhd", p, vf).reshape(n, nq * D).to(q.dtype)
+
+
+def _paged_rows(pages: torch.Tensor, table: torch.Tensor, n: int) -> torch.Tensor:
+    """The first n positions of a sequence's pages, [n, nkv, D]."""
+    ps = pages.shape[2]
+    x = pages[table[: (n + ps - 1) // ps].long()]
+    return x.transpose(1, 2).reshape(-1, pages.shape[1], pages.shape[3])[:n]
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None
+                     ) -> torch.Tensor:
+    _check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and k.shape[2] == q.shape[2],
+           "k and v must be [rows, kv heads, head_dim] with the queries' head_dim")
+    _check_heads(q.shape[1], k.shape[1])
+    _check(cu_seqlens_k is not None or k.shape[0] == q.shape[0],
+           "k has other rows than q: give cu_seqlens_k")
+    cu_k = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
+    for c in (cu_seqlens, cu_k):
+        _check(c.dtype == torch.int32 and c.numel() == cu_seqlens.numel() >= 1,
+               "cu_seqlens must hold n + 1 int32 offsets")
+    out = torch.zeros(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
+    cq, ck = cu_seqlens.tolist(), cu_k.tolist()
+    for i in range(len(cq) - 1):
+        if cq[i + 1] > cq[i] and ck[i + 1] > ck[i]:
+            out[cq[i]:cq[i + 1]] = _causal_rows(q[cq[i]:cq[i + 1]], k[ck[i]:ck[i + 1]],
+                                                v[ck[i]:ck[i + 1]], scale)
+    return out
+
+
+def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                            page_table: torch.Tensor, seq_lens: torch.Tensor,
+                            cu_seqlens: torch.Tensor, scale: Optional[float] = None
+                            ) -> torch.Tensor:
+    _check(q.dim() == 3, "q must be [rows, heads, head_dim]")
+    _check_pool(k_pages, v_pages, q.shape[2])
+    _check_heads(q.shape[1], k_pages.shape[1])
+    n = cu_seqlens.numel() - 1
+    for t in (page_table, seq_lens, cu_seqlens):
+        _check(t.dtype == torch.int32, "page_table, seq_lens and cu_seqlens must be int32")
+    _check(page_table.dim() == 2 and page_table.shape[0] == n and seq_lens.numel() == n,
+           f"page_table and seq_lens must have a row for each of the {n} sequences")
+    out = torch.zeros(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
+    cq = cu_seqlens.tolist()
+    for i in range(n):
+        m = int(seq_lens[i])
+        if cq[i + 1] > cq[i] and m > 0:
+            out[cq[i]:cq[i + 1]] = _causal_rows(q[cq[i]:cq[i + 1]],
+                                                _paged_rows(k_pages, page_table[i], m),
+                                                _paged_rows(v_pages, page_table[i], m), scale)
+    return out
+
+
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           page_table: torch.Tensor, seq_lens: torch.Tensor,
+                           scale: Optional[float] = None) -> torch.Tensor:
+    cu = torch.arange(q.shape[0] + 1, dtype=torch.int32)
+    return paged_prefill_attention(q, k_pages, v_pages, page_table, seq_lens, cu, scale)
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be [rows, vocab]")
+    _check(logits.dtype in (torch.bfloat16, torch.float16, torch.float32),
+           "logits must be bf16, fp16 or fp32")
+    R, V = logits.shape
+    _check(ids.dtype == torch.int64 and ids.numel() == R,
+           "ids must be a contiguous int64 tensor, one per row")
+    _check(0 <= top_k <= min(32, V), "top_k must be at most 32 and the vocabulary")
+    ls = torch.log_softmax(logits.float(), -1)
+    p = ls.exp()
+    entropy = -(torch.where(p == 0, torch.zeros_like(p), p * ls)).sum(-1)
+    ok = (ids >= 0) & (ids < V)
+    lp = ls.gather(1, ids.clamp(0, V - 1)[:, None])[:, 0].masked_fill(~ok, float("nan"))
+    # stable: equal logits in index order; a NaN sorts first
+    top = torch.sort(logits.float() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    return lp, entropy, top, ls.gather(1, top)

@@ -773,6 +773,10 @@ void ipc_close(int64_t ptr) { cudaIpcCloseMemHandle(reinterpret_cast<void*>(ptr)
 
 }  // namespace
 
+namespace afd {
+void bind_ragged(pybind11::module& m);  // bindings_ragged.cpp
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "afd_demo_b200 sm_100a kernels";
   m.def("num_sms", &num_sms);
@@ -804,4 +808,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ipc_handle", &ipc_handle);
   m.def("ipc_open", &ipc_open);
   m.def("ipc_close", &ipc_close);
+  afd::bind_ragged(m);
 }

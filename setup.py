@@ -25,7 +25,8 @@ if os.environ.get("AFD_BOUNDS_CHECK"):
     NVCC_FLAGS.append("-DAFD_BOUNDS_CHECK=1")
 
 SOURCES = ["bindings.cpp", "gemm_tcgen05.cu", "gemm_tm.cu", "kernels.cu", "attention.cu",
-           "attention_tc.cu", "decode_attention_tc.cu", "noalloc.cu"]
+           "attention_tc.cu", "decode_attention_tc.cu", "noalloc.cu", "bindings_ragged.cpp",
+           "norm_rope_paged.cu", "packed_attention.cu", "paged_decode.cu", "token_logprobs.cu"]
 
 setup(
     name="afd_demo_b200",
