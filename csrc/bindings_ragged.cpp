@@ -7,12 +7,17 @@
 // builder crashes where the extension carries its own copy of the C++ runtime.
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "ragged.h"
 
@@ -40,6 +45,24 @@ int elem16(const at::Tensor& t, const char* what) {
 void check_like(const at::Tensor& t, const at::Tensor& like, const char* what) {
   TORCH_CHECK_VALUE(t.device() == like.device() && t.scalar_type() == like.scalar_type(), what,
               " must be on the queries' device and of their type");
+}
+
+int num_sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+
+// Zeroed counters that the kernels leave zeroed: one buffer for each stream
+// (calls on one stream follow one another), kept for good. Inside a stream
+// capture the call gets zeros of its own, set again at every replay, so that
+// graphs may be replayed on any stream.
+at::Tensor zeroed_counters(const at::Tensor& like, int64_t n) {
+  const auto opt = at::TensorOptions().device(like.device()).dtype(at::kInt);
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return at::zeros({n}, opt);
+  static std::mutex mu;
+  static auto* pool = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
+  std::lock_guard<std::mutex> lock(mu);
+  at::Tensor& t = (*pool)[{like.device().index(), stream()}];
+  if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 1024)}, opt);
+  return t;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -98,6 +121,8 @@ void take_pool(Args& a, const at::Tensor& k_pages, const at::Tensor& v_pages,
 }
 
 float scale_of(c10::optional<double> scale, int D) {
+  TORCH_CHECK_VALUE(!scale.has_value() || (*scale > 0 && std::isfinite(*scale)),
+                    "scale must be positive");
   return scale.has_value() ? (float)*scale : 1.f / std::sqrt((float)D);
 }
 
@@ -193,7 +218,9 @@ at::Tensor packed_attention(const at::Tensor& q_in, const at::Tensor& k_in, cons
   a.v_row = v.stride(0);
   a.Tk = (int)k.size(0);
   a.cu_k = cu_k.data_ptr<int>();
-  check_rc(launch_packed_attention(a, stream()), "packed_attention");
+  const at::Tensor counter = zeroed_counters(q, 1);
+  a.counter = counter.data_ptr<int>();
+  check_rc(launch_packed_attention(a, num_sms(), stream()), "packed_attention");
   return out;
 }
 
@@ -214,7 +241,9 @@ at::Tensor paged_prefill_attention(const at::Tensor& q_in, const at::Tensor& k_p
   a.k_pages = k_pages.data_ptr();
   a.v_pages = v_pages.data_ptr();
   a.seq_lens = seq_lens.data_ptr<int>();
-  check_rc(launch_packed_attention(a, stream()), "paged_prefill_attention");
+  const at::Tensor counter = zeroed_counters(q, 1);
+  a.counter = counter.data_ptr<int>();
+  check_rc(launch_packed_attention(a, num_sms(), stream()), "paged_prefill_attention");
   return out;
 }
 

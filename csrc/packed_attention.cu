@@ -1,7 +1,46 @@
-// Causal attention of packed queries over packed keys or over the paged cache.
+// Causal GQA attention of packed queries over packed keys or over the paged
+// cache, on the 5th-generation tensor cores.
 //
-// out[r, h] = sum_j p_j v_j,  p = softmax over the visible keys j <= pos(r) of
-// q[r, h] . k_j * scale, with h's kv head h / (nq / nkv).
+//   out[r, h] = sum_j p_j v_j,  p = softmax over the visible keys j <= pos(r)
+//               of q[r, h] . k_j * scale, with h's kv head h / G, G = nq / nkv
+//
+// The G heads that share a kv head share every K and V row, so a row tile of
+// the first product holds 128 / G tokens x G heads of one sequence: a short
+// prompt still fills the tile, and only the keys that its few tokens see are
+// visited (a 128-token tile of one head would spend half of its last key tile
+// on the mask). One block is two such row tiles, A and B, of consecutive
+// tokens, which share every K and V tile in shared memory.
+//
+// Steps of 64 keys. For row tile X, S_X = Q_X K^T (M 128, N 64) and
+// O_X += P_X V (P from TMEM) accumulate in TMEM; S and P of consecutive steps
+// take two buffers in turn, so the product S_X(i+1) is finished while the
+// softmax of step i still runs and the softmax warps never wait for the tensor
+// core's latency. With one buffer (S of 128 keys, P over it) that chain
+// softmax -> P V -> S bounded the step.
+//
+//   warp 0      work items, TMA producer: Q tiles, then K and V rings of 4 steps
+//   warp 1      TMEM owner (512 columns) and MMA issuer
+//   warps 2..5  softmax of row tile A, warps 6..9 of row tile B (a row a thread)
+//
+// Issue order of the MMA warp, i the step:  P_A(i) V | S_B(i+1) | P_B(i) V |
+// S_A(i+2).  S_X(i+2) overwrites P_X(i): it waits for the commit of P_X(i) V,
+// half a step old by then.
+//
+// The running maximum is raised only when a row's maximum grows by more than 8
+// (in powers of two): P then holds values up to 256, exact in the ratio O / l,
+// and O is rescaled in TMEM only in such steps. P is rounded to the input type
+// for the second product; maxima, sums and both accumulators are fp32.
+//
+// TMEM columns: S_A [0,128), S_B [128,256) (two buffers of 64; P over the first
+// 32 of each), O_A [256,256+D), O_B [384,384+D).
+//
+// Persistent CTAs take items (block of a sequence, kv head) in turn from a
+// counter that wraps to zero with the last fetch of a launch. Slot s of the
+// blocks belongs to the last sequence i with cu[i] / TB + i <= s: that leaves
+// at least ceil(length / TB) slots for each sequence without a prefix sum over
+// lengths, and a sequence's longest-running blocks come first.
+
+#include <string.h>
 
 #include "ragged.cuh"
 
@@ -9,86 +48,599 @@ namespace afd {
 
 namespace {
 
-// One warp per (query row, head); the lanes split the head dim, and each key
-// updates the running maximum and sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) packed_attention_kernel(PackedAttnArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x % 32;
-  const long long gw = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-  if (gw >= (long long)a.T * a.nq) return;
-  const int row = (int)(gw / a.nq), h = (int)(gw % a.nq), kvh = h / (a.nq / a.nkv);
-  constexpr int E = D / 32;
-  const T* q = reinterpret_cast<const T*>(a.q) + (size_t)row * a.q_row + (size_t)h * D;
-  float qv[E], o[E];
-  for (int i = 0; i < E; ++i) {
-    qv[i] = to_f(q[lane * E + i]) * a.scale;
-    o[i] = 0.f;
-  }
-  // the last sequence that starts at or before this row
-  int lo = 0, hi = a.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.cu_q[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  const int q0 = a.cu_q[lo], q1 = min(a.cu_q[lo + 1], a.T);
-  int len = 0, k0 = 0;
-  if (a.n_seqs > 0 && row >= q0 && row < q1) {
-    if (a.paged) {
-      len = checked_len(a.seq_lens[lo], a.max_pages * a.page_size, a.status, 211);
-    } else {
-      k0 = min(max(a.cu_k[lo], 0), a.Tk);
-      len = min(max(a.cu_k[lo + 1], k0), a.Tk) - k0;
-      if (k0 != a.cu_k[lo] || k0 + len != a.cu_k[lo + 1])
-        report_status(a.status, kBoundsViolation, 212);
-    }
-  }
-  const int pos = len > 0 ? len - (q1 - row) : -1;
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j <= pos; ++j) {
-    const T *k, *v;
-    bool ok = true;
-    if (a.paged) {
-      const int page = a.page_table[(size_t)lo * a.table_row + j / a.page_size];
-      ok = page >= 0 && page < a.num_pages;
-      const size_t at = (size_t)(ok ? page : 0) * a.page_stride +
-                        ((size_t)kvh * a.page_size + j % a.page_size) * D;
-      k = reinterpret_cast<const T*>(a.k_pages) + at;
-      v = reinterpret_cast<const T*>(a.v_pages) + at;
-      if (!ok) report_status(a.status, kBoundsViolation, 213);
-    } else {
-      k = reinterpret_cast<const T*>(a.k) + (size_t)(k0 + j) * a.k_row + (size_t)kvh * D;
-      v = reinterpret_cast<const T*>(a.v) + (size_t)(k0 + j) * a.v_row + (size_t)kvh * D;
-    }
-    float s = 0.f;
-    for (int i = 0; i < E; ++i) s += qv[i] * (ok ? to_f(k[lane * E + i]) : 0.f);
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float m_new = fmaxf(m, s);
-    const float c = m_new == -INFINITY ? 1.f : __expf(m - m_new);
-    const float p = m_new == -INFINITY ? 0.f : __expf(s - m_new);
-    l = l * c + p;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * c + p * (ok ? to_f(v[lane * E + i]) : 0.f);
-    m = m_new;
-  }
-  T* out = reinterpret_cast<T*>(a.out) + ((size_t)row * a.nq + h) * D;
-  for (int i = 0; i < E; ++i) out[lane * E + i] = from_f<T>(l > 0.f ? o[i] / l : 0.f);
+constexpr int kRows = 128;    // rows of a tile (TMEM lanes)
+constexpr int kKeys = 64;     // keys of a step
+constexpr int kStages = 4;    // K and V ring depth
+constexpr int kThreads = 320;
+
+struct Item {
+  int steps;    // 64-key steps; 0: no key; -1: no more work
+  int row0;     // query row of the block's first token
+  int tokens;   // tokens of the sequence from there on (may exceed the block)
+  int pos0;     // position of the first token
+  int kvh;
+};
+
+// Two fp32 lanes per instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
 }
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 lanes x 32 bit, 64 consecutive columns per thread: two loads, one wait.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]),
+        "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+        "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]),
+        "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_st16_raw(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32"
+      " [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+        "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+        "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// D (TMEM) (+)= A (TMEM, 128 lanes x 16 elements) x B (shared memory).
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t idesc16(int M, int N, bool b_mn_major) {
+  uint32_t d = umma_idesc_bf16(M, N, b_mn_major);
+  // formats of A (bits 7..9) and B (10..12): 1 = bf16, 0 = fp16
+  if (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) d &= ~((1u << 7) | (1u << 10));
+  return d;
+}
+
+template <int D>
+struct Smem {
+  static constexpr int kBoxes = D / 64;                 // 128-byte wide boxes of a row
+  static constexpr int kQTile = kRows * D * 2;          // one row tile
+  static constexpr int kQBox = kRows * 128;
+  static constexpr int kKvTile = kKeys * D * 2;         // K or V of one step
+  static constexpr int kKvBox = kKeys * 128;
+  static constexpr int kBytes = 2 * kQTile + 2 * kStages * kKvTile + 1024 /*align*/ + 512;
+};
 
 }  // namespace
 
-int launch_packed_attention(const PackedAttnArgs& a, cudaStream_t s) {
-  if (a.T == 0) return 0;
-  const dim3 grid((unsigned)(((long long)a.T * a.nq + 3) / 4));
-  cudaError_t e;
-  if (a.elem == kElemBf16)
-    e = a.D == 128 ? launch_k(packed_attention_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, s, a)
-                   : launch_k(packed_attention_kernel<__nv_bfloat16, 64>, grid, dim3(128), 0, s, a);
-  else
-    e = a.D == 128 ? launch_k(packed_attention_kernel<__half, 128>, grid, dim3(128), 0, s, a)
-                   : launch_k(packed_attention_kernel<__half, 64>, grid, dim3(128), 0, s, a);
+template <typename T, int D, bool kPaged>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_attention_kernel(const __grid_constant__ CUtensorMap tq,
+                            const __grid_constant__ CUtensorMap tk,
+                            const __grid_constant__ CUtensorMap tv, PackedAttnArgs a, int tok1,
+                            int n_items, int box_rows) {
+  using L = Smem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                                  // row tile X at X * kQTile
+  uint8_t* k_s = q_s + 2 * L::kQTile;
+  uint8_t* v_s = k_s + kStages * L::kKvTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + kStages * L::kKvTile);
+  uint64_t* k_full = bars;                              // [kStages]
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* s_full = v_empty + kStages;                 // [2 row tiles][2 buffers]
+  uint64_t* p_full = s_full + 4;
+  uint64_t* pv_done = p_full + 4;
+  uint64_t* o_free = pv_done + 4;                       // [2 row tiles]
+  uint64_t* q_full = o_free + 2;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* item_full = q_empty + 1;                    // [2]
+  uint64_t* item_empty = item_full + 2;                 // [2]
+  Item* items = reinterpret_cast<Item*>(item_empty + 2);  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int G = a.nq / a.nkv;
+  const int block_tokens = 2 * tok1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&o_free[i], 4);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 9);  // the MMA thread and 8 softmax warps
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tq);
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    // -------------------------------------------- work items, TMA producer
+    auto cu_q = [&](int i) { return min(max(a.cu_q[i], 0), a.T); };
+    int g = 0, qi = 0, published = 0;
+    bool ok = true;
+    int item = blockIdx.x;
+    while (item < n_items) {
+      const int slot = item / a.nkv, kvh = item % a.nkv;
+      // the last sequence whose first slot is at or before `slot`; sequence
+      // n_seqs stands for the rows past the last offset
+      int lo = 0, hi = a.n_seqs + 1;
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + step * (lane + 1);
+        const bool le = at < hi && cu_q(at) / block_tokens + at <= slot;
+        const int n = __popc(__ballot_sync(0xffffffffu, le));
+        hi = min(hi, lo + step * (n + 1));
+        lo += step * n;
+      }
+      Item w;
+      w.kvh = kvh;
+      const int q0 = cu_q(lo), q1 = lo < a.n_seqs ? max(cu_q(lo + 1), q0) : a.T;
+      const int blocks = (q1 - q0 + block_tokens - 1) / block_tokens;
+      const int block = blocks - 1 - (slot - (q0 / block_tokens + lo));
+      int k0 = 0, len = 0;
+      if (lo < a.n_seqs && block >= 0) {
+        if (lane == 0 && (a.cu_q[lo] != q0 || a.cu_q[lo + 1] != q1))
+          report_status(a.status, kBoundsViolation, 210);
+        if (kPaged) {
+          len = checked_len(a.seq_lens[lo], a.max_pages * a.page_size, a.status, 211);
+        } else {
+          const int c0 = a.cu_k[lo], c1 = a.cu_k[lo + 1];
+          k0 = min(max(c0, 0), a.Tk);
+          len = min(max(c1, k0), a.Tk) - k0;
+          if (lane == 0 && (k0 != c0 || k0 + len != c1))
+            report_status(a.status, kBoundsViolation, 212);
+        }
+      }
+      w.row0 = q0 + block * block_tokens;
+      w.tokens = q1 - w.row0;
+      w.pos0 = len - (q1 - w.row0);
+      const int last = len > 0 ? w.pos0 + min(w.tokens, block_tokens) - 1 : -1;
+      w.steps = last >= 0 ? last / kKeys + 1 : 0;
+      if (block >= 0 && ok) {
+        // hand the item to the other warps
+        const int ib = published & 1;
+        if (published >= 2 &&
+            !__all_sync(0xffffffffu, mbar_wait(&item_empty[ib], ((published >> 1) - 1) & 1,
+                                               abort_flag, a.status, 230)))
+          ok = false;
+        if (ok && lane == 0) {
+          items[ib] = w;
+          mbar_arrive(&item_full[ib]);
+        }
+        ++published;
+        if (ok && lane == 0 && w.steps > 0) {
+          if (qi > 0 && !mbar_wait(q_empty, (qi - 1) & 1, abort_flag, a.status, 231)) ok = false;
+          if (ok) {
+            mbar_arrive_expect_tx(q_full, 2 * L::kBoxes * G * tok1 * 128);
+            for (int x = 0; x < 2; ++x)
+              for (int c = 0; c < L::kBoxes; ++c)
+                tma_load_3d(q_s + x * L::kQTile + c * L::kQBox, &tq, q_full, c * 64, kvh * G,
+                            w.row0 + x * tok1);
+            ++qi;
+          }
+          const int* table = kPaged ? a.page_table + (size_t)lo * a.table_row : nullptr;
+          for (int i = 0; ok && i < w.steps; ++i, ++g) {
+            const int st = g % kStages;
+            const uint32_t phase = ((g / kStages) - 1) & 1;
+            const int key0 = i * kKeys;
+            // rows past the sequence's end are not fetched (a box at a time)
+            const int boxes = kPaged ? (min(kKeys, len - key0) + box_rows - 1) / box_rows : 1;
+            const uint32_t bytes = L::kBoxes * boxes * box_rows * 128;
+            for (int kv = 0; kv < 2; ++kv) {
+              uint64_t* full = kv == 0 ? &k_full[st] : &v_full[st];
+              if (g >= kStages && !mbar_wait(kv == 0 ? &k_empty[st] : &v_empty[st], phase,
+                                             abort_flag, a.status, 232 + kv)) {
+                ok = false;
+                break;
+              }
+              uint8_t* dst = (kv == 0 ? k_s : v_s) + st * L::kKvTile;
+              const CUtensorMap* map = kv == 0 ? &tk : &tv;
+              mbar_arrive_expect_tx(full, bytes);
+              if (kPaged) {
+                for (int r = 0; r < boxes; ++r) {
+                  const int key = key0 + r * box_rows;
+                  const int page = table[key / a.page_size];
+                  if (page < 0 || page >= a.num_pages)  // the copy fills with zeros
+                    report_status(a.status, kBoundsViolation, 213);
+                  for (int c = 0; c < L::kBoxes; ++c)
+                    tma_load_3d(dst + c * L::kKvBox + r * box_rows * 128, map, full, c * 64,
+                                kvh * a.page_size + key % a.page_size, page);
+                }
+              } else {
+                for (int c = 0; c < L::kBoxes; ++c)
+                  tma_load_3d(dst + c * L::kKvBox, map, full, c * 64, kvh, k0 + key0);
+              }
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      }
+      // the next item; with the last fetch of the launch the counter is zero again
+      if (lane == 0) item = (int)gridDim.x + (int)atomicInc(
+          reinterpret_cast<unsigned*>(a.counter), (unsigned)n_items - 1);
+      item = __shfl_sync(0xffffffffu, item, 0);
+    }
+    if (ok) {
+      const int ib = published & 1;
+      if (published >= 2 &&
+          !__all_sync(0xffffffffu, mbar_wait(&item_empty[ib], ((published >> 1) - 1) & 1,
+                                             abort_flag, a.status, 234)))
+        ok = false;
+      if (ok && lane == 0) {
+        items[ib].steps = -1;
+        mbar_arrive(&item_full[ib]);
+      }
+    }
+    if (lane == 0) {
+      // every load issued must land before the CTA exits (after an abort the
+      // other warps may not have waited for it)
+      volatile int no_abort = 0;
+      if (qi > 0) mbar_wait(q_full, (qi - 1) & 1, &no_abort, nullptr, 235, 100000000ull);
+      if (!ok) {
+        for (int j = max(0, g + 1 - kStages); j <= g; ++j) {
+          mbar_wait(&k_full[j % kStages], (j / kStages) & 1, &no_abort, nullptr, 236, 100000000ull);
+          mbar_wait(&v_full[j % kStages], (j / kStages) & 1, &no_abort, nullptr, 237, 100000000ull);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      const uint32_t idesc_s = idesc16<T>(kRows, kKeys, false);
+      const uint32_t idesc_pv = idesc16<T>(kRows, D, true);
+      const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
+      int g = 0, it = 0, taken = 0, n = 0;
+      bool ok = true;
+      auto issue_s = [&](int x, int i) {
+        const int idx = g + i, st = idx % kStages, buf = idx & 1;
+        if (x == 0 && !mbar_wait(&k_full[st], (idx / kStages) & 1, abort_flag, a.status, 240))
+          return false;
+        if (idx >= 2 && !mbar_wait(&pv_done[2 * x + buf], ((idx >> 1) - 1) & 1, abort_flag,
+                                   a.status, 241))
+          return false;
+        tc_fence_after();
+        const uint32_t qa = q_base + x * L::kQTile, ka = k_base + st * L::kKvTile;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(tmem + x * 128 + buf * 64,
+                    umma_desc_sw128(qa + (kk / 4) * L::kQBox + (kk % 4) * 32),
+                    umma_desc_sw128(ka + (kk / 4) * L::kKvBox + (kk % 4) * 32), idesc_s,
+                    kk > 0);
+        umma_commit(&s_full[2 * x + buf]);
+        if (x == 1) umma_commit(&k_empty[st]);
+        if (x == 1 && i == n - 1) umma_commit(q_empty);
+        return true;
+      };
+      auto issue_pv = [&](int x, int i) {
+        const int idx = g + i, st = idx % kStages, buf = idx & 1;
+        if (x == 0 && !mbar_wait(&v_full[st], (idx / kStages) & 1, abort_flag, a.status, 242))
+          return false;
+        if (!mbar_wait(&p_full[2 * x + buf], (idx >> 1) & 1, abort_flag, a.status, 243))
+          return false;
+        if (i == 0 && it > 0 && !mbar_wait(&o_free[x], (it - 1) & 1, abort_flag, a.status, 244))
+          return false;
+        tc_fence_after();
+        const uint32_t va = v_base + st * L::kKvTile;
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + buf * 64 + kk * 8,
+                  umma_desc_sw128_mn(va + kk * 2048, L::kKvBox, 1024), idesc_pv,
+                  (i > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&pv_done[2 * x + buf]);
+        if (x == 1) umma_commit(&v_empty[st]);
+        return true;
+      };
+      while (ok) {
+        const int ib = taken & 1;
+        if (!mbar_wait(&item_full[ib], (taken >> 1) & 1, abort_flag, a.status, 245))
+          break;
+        n = items[ib].steps;
+        mbar_arrive(&item_empty[ib]);
+        ++taken;
+        if (n < 0) break;
+        if (n == 0) continue;
+        if (!mbar_wait(q_full, it & 1, abort_flag, a.status, 246)) break;
+        ok = issue_s(0, 0) && issue_s(1, 0) && (n == 1 || issue_s(0, 1));
+        for (int i = 0; ok && i < n; ++i)
+          ok = issue_pv(0, i) && (i + 1 >= n || issue_s(1, i + 1)) && issue_pv(1, i) &&
+               (i + 2 >= n || issue_s(0, i + 2));
+        g += n;
+        ++it;
+      }
+    }
+  } else {
+    // ------------------------------------------- softmax, O, output rows
+    const int x = (warp - 2) / 4;         // row tile of this warp group
+    const int qq = warp & 3;              // TMEM lane quarter of this warp
+    const int row = qq * 32 + lane;
+    const int tok = x * tok1 + row / G;   // this row's token in the block
+    const bool has_token = row < tok1 * G;
+    const int tok_first = x * tok1 + (qq * 32) / G;  // of the warp's first row
+    const uint32_t lane_off = (uint32_t)(qq * 32) << 16;
+    const uint32_t t_o = tmem + 256 + x * 128 + lane_off;
+    const float scale_log2 = a.scale * 1.4426950408889634f;
+    int g = 0, taken = 0;
+    bool ok = true;
+    // TMEM accesses are warp-collective: every branch around them is
+    // warp-uniform
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, int where) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status, where));
+      return ok;
+    };
+    while (ok) {
+      const int ib = taken & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[ib], (taken >> 1) & 1, abort_flag,
+                                             a.status, 250));
+      if (!ok) break;
+      const Item w = items[ib];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[ib]);
+      ++taken;
+      if (w.steps < 0) break;
+      // rows past the sequence's end (never stored) see what its last row sees
+      const int len = w.pos0 + w.tokens;
+      const int pos = min(w.pos0 + tok, len - 1);
+      const int warp_pos0 = min(w.pos0 + tok_first, len - 1);
+      float m = -INFINITY;
+      float2 l2 = make_float2(0.f, 0.f);
+      for (int i = 0; i < w.steps; ++i, ++g) {
+        const int buf = g & 1, key0 = i * kKeys;
+        const uint32_t t_s = tmem + x * 128 + buf * 64 + lane_off;
+        if (!wait_all(&s_full[2 * x + buf], (g >> 1) & 1, 251)) break;
+        tc_fence_after();
+        float s[kKeys];
+        tmem_ld64(t_s, s);
+        // below the diagonal for every row of this warp: nothing to mask
+        if (key0 + kKeys - 1 > warp_pos0) {
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k)
+            if (key0 + k > pos) s[k] = -INFINITY;
+          if (x == 0 && key0 + kKeys > len) {
+            // rows past the sequence's end belong to others or to nobody: zero
+            // V there, so that P = 0 meets finite values
+            const int st = g % kStages;
+            if (!wait_all(&v_full[st], (g / kStages) & 1, 252)) break;
+            const int r = row / 2;
+            if (key0 + r >= len) {
+              uint8_t* vr = v_s + st * L::kKvTile + r * 128 + (row & 1) * 64;
+#pragma unroll
+              for (int c = 0; c < L::kBoxes; ++c)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                  *reinterpret_cast<uint4*>(vr + c * L::kKvBox + u * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int k = 4; k < kKeys - 4; k += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[k + 2 * e], s[k + 2 * e + 1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[kKeys - 4 + e]);
+        const float rmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale_log2;
+        const bool grow = rmax > m + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? rmax : m;
+          if (i > 0) {
+            // O holds steps 0 .. i-1 once P(i-1) V is done
+            if (!wait_all(&pv_done[2 * x + (buf ^ 1)], ((g - 1) >> 1) & 1, 253)) break;
+            tc_fence_after();
+            const float alpha = grow ? exp2_approx(m - m_new) : 1.f;
+            l2.x *= alpha;
+            l2.y *= alpha;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld16(t_o + c * 16, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tmem_st16(t_o + c * 16, o);
+            }
+          }
+          m = m_new;
+        }
+        // p = 2^(s scale log2(e) - m); a masked s = -inf gives 0, also in a row
+        // that has seen no key yet (m = -inf)
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+        const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(neg_m, neg_m);
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 p = fma2(make_float2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), sc2, nm2);
+            p.x = exp2_approx(p.x);
+            p.y = exp2_approx(p.y);
+            l2 = add2(l2, p);
+            pk[e] = pack2<T>(p.x, p.y);
+          }
+          tmem_st16_raw(t_s + c * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * x + buf]);
+      }
+      if (!ok) break;
+      const bool valid = has_token && tok < w.tokens;
+      T* dst = reinterpret_cast<T*>(a.out) +
+               ((size_t)(w.row0 + tok) * a.nq + w.kvh * G + row % G) * D;
+      const float l = l2.x + l2.y;
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (w.steps > 0) {
+        if (!wait_all(&pv_done[2 * x + ((g - 1) & 1)], ((g - 1) >> 1) & 1, 254)) break;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (w.steps > 0) {
+          tmem_ld32(t_o + c * 32, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 v;
+            // a row that saw no key: exact zeros whatever O holds
+            v.x = l > 0.f ? pack2<T>(o[8 * e + 0] * inv, o[8 * e + 1] * inv) : 0u;
+            v.y = l > 0.f ? pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv) : 0u;
+            v.z = l > 0.f ? pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv) : 0u;
+            v.w = l > 0.f ? pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv) : 0u;
+            *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = v;
+          }
+        }
+      }
+      if (w.steps > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[x]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ============================================================ host side ===
+
+template <typename T, int D, bool kPaged>
+static int launch_one(const PackedAttnArgs& a, int num_sms, const CUtensorMap& tq,
+                      const CUtensorMap& tk, const CUtensorMap& tv, int tok1, int box_rows,
+                      cudaStream_t s) {
+  const auto kern = packed_attention_kernel<T, D, kPaged>;
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
+  if (e != cudaSuccess) return 4000 + (int)e;
+  const long long items = ((long long)a.T / (2 * tok1) + a.n_seqs + 1) * a.nkv;
+  if (items > 0x3fffffff) return 1;
+  const int grid = (int)(items < num_sms ? items : num_sms);
+  e = launch_k(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, s, tq, tk, tv, a, tok1,
+               (int)items, box_rows);
   return e == cudaSuccess ? 0 : 4000 + (int)e;
+}
+
+int launch_packed_attention(const PackedAttnArgs& a, int num_sms, cudaStream_t s) {
+  if (a.T == 0) return 0;
+  if (!a.paged && a.Tk == 0) {  // no key anywhere
+    const cudaError_t e = cudaMemsetAsync(a.out, 0, (size_t)a.T * a.nq * a.D * 2, s);
+    return e == cudaSuccess ? 0 : 4000 + (int)e;
+  }
+  const int G = a.nq / a.nkv, tok1 = kRows / G;
+  CUtensorMap tq, tk, tv;
+  const uint64_t e2 = 2;  // bytes of an element
+  {  // q [T, nq, D]: a box is tok1 tokens x the G heads of a kv head
+    const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.nq, (uint64_t)a.T};
+    const uint64_t str[2] = {a.D * e2, (uint64_t)a.q_row * e2};
+    const uint32_t box[3] = {64, (uint32_t)G, (uint32_t)tok1};
+    if (int e = encode_map16(&tq, a.q, a.elem, 3, dims, str, box)) return e;
+  }
+  int box_rows = kKeys;
+  if (a.paged) {
+    // pool [pages, nkv * page_size, D]: the largest box that no page ends inside
+    while (a.page_size % box_rows) box_rows /= 2;
+    const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.nkv * a.page_size,
+                              (uint64_t)a.num_pages};
+    const uint64_t str[2] = {a.D * e2, (uint64_t)a.page_stride * e2};
+    const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+    if (int e = encode_map16(&tk, a.k_pages, a.elem, 3, dims, str, box)) return e;
+    if (int e = encode_map16(&tv, a.v_pages, a.elem, 3, dims, str, box)) return e;
+  } else {
+    const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.nkv, (uint64_t)a.Tk};
+    const uint32_t box[3] = {64, 1, (uint32_t)kKeys};
+    const uint64_t kstr[2] = {a.D * e2, (uint64_t)a.k_row * e2};
+    const uint64_t vstr[2] = {a.D * e2, (uint64_t)a.v_row * e2};
+    if (int e = encode_map16(&tk, a.k, a.elem, 3, dims, kstr, box)) return e;
+    if (int e = encode_map16(&tv, a.v, a.elem, 3, dims, vstr, box)) return e;
+  }
+#define AFD_PACKED(T, D)                                                                    \
+  (a.paged ? launch_one<T, D, true>(a, num_sms, tq, tk, tv, tok1, box_rows, s)              \
+           : launch_one<T, D, false>(a, num_sms, tq, tk, tv, tok1, box_rows, s))
+  if (a.elem == kElemBf16)
+    return a.D == 128 ? AFD_PACKED(__nv_bfloat16, 128) : AFD_PACKED(__nv_bfloat16, 64);
+  return a.D == 128 ? AFD_PACKED(__half, 128) : AFD_PACKED(__half, 64);
+#undef AFD_PACKED
 }
 
 }  // namespace afd

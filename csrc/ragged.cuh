@@ -3,6 +3,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "ragged.h"
 
@@ -45,6 +47,38 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+// Tensor map over 16-bit elements with 128-byte swizzle, zeros out of bounds:
+// dims[0] innermost, byte strides of dims 1 .., box[0] = 64 elements.
+inline int encode_map16(CUtensorMap* m, const void* base, int elem, int rank, const uint64_t* dims,
+                        const uint64_t* strides, const uint32_t* box) {
+  typedef CUresult (*Fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                         const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                         CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                         CUtensorMapFloatOOBfill);
+  static const Fn fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    const cudaError_t e =
+        cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<Fn>(p)
+                                                                : nullptr;
+  }();
+  if (fn == nullptr) return 50;
+  cuuint64_t d[4], st[3];
+  cuuint32_t bx[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  const CUresult r =
+      fn(m, elem == kElemBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         rank, const_cast<void*>(base), d, st, bx, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 100 + (int)r;
 }
 
 // A sequence length read from the device: values outside [0, most] are

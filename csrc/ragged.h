@@ -68,11 +68,12 @@ struct PackedAttnArgs {
   int num_pages, page_size, max_pages;
   void* out;                // [T, nq, D]
   int nq, nkv, D;
-  float scale;
+  float scale;              // > 0
   int elem;
   int* status;
+  int* counter;             // [1], zero; left zero
 };
-int launch_packed_attention(const PackedAttnArgs& a, cudaStream_t s);
+int launch_packed_attention(const PackedAttnArgs& a, int num_sms, cudaStream_t s);
 
 // Per-head RMSNorm and RoPE of the q and k heads of a packed qkv projection.
 // q goes to q_out; k to k_out [T, nkv, D], or with the pool given, k and v to
