@@ -170,7 +170,14 @@ at::Tensor paged_decode_attention(const at::Tensor& q_in, const at::Tensor& k_pa
   a.out = out.data_ptr();
   a.scale = scale_of(scale, a.D);
   a.status = status_ptr(status, q);
-  check_rc(launch_paged_decode(a, stream()), "paged_decode_attention");
+  const int grid = num_sms();
+  const int64_t parts = paged_decode_part_rows(a.nq, a.nkv, grid);
+  const at::Tensor ws = at::empty({parts * (a.D + 2)}, q.options().dtype(at::kFloat));
+  const at::Tensor counters = zeroed_counters(q, grid);
+  a.o_part = ws.data_ptr<float>();
+  a.ml_part = reinterpret_cast<float2*>(a.o_part + parts * a.D);
+  a.counters = counters.data_ptr<int>();
+  check_rc(launch_paged_decode(a, grid, stream()), "paged_decode_attention");
   return out;
 }
 

@@ -1,7 +1,38 @@
-// Attention of one new token per sequence over the paged KV cache.
+// Attention of one new token per sequence over the paged KV cache, split over
+// the cache's length and joined in the same launch.
 //
-// out[b, h] = sum_j p_j v_j, p = softmax over j < seq_lens[b] of
-// q[b, h] . k_j * scale, with h's kv head h / (nq / nkv).
+//   out[b, h] = sum_j p_j v_j, p = softmax over j < seq_lens[b] of
+//   q[b, h] . k_j * scale, with h's kv head h / G, G = nq / nkv
+//
+// What bounds it is reading K and V once: 4 G flops an element of K or V, a
+// hundredth of what the tensor cores have over the HBM's rate. So the layout serves
+// the loads, and the products use the warp-level MMA, whose operands and
+// results stay in the registers of one warp: no barrier between warps, no
+// round trip through TMEM, and a running maximum of each warp's own.
+//
+// A warp takes blocks of 16 keys (a page holds a whole number of them) through
+// a ring of its own in shared memory, which its lane 0 refills by TMA as soon as
+// the block is consumed. For a block, with the keys as the rows of the MMA:
+//
+//   S^T [16 keys x 8 heads]  = K [16 x D] Q^T          (K by ldmatrix)
+//   O^T [D x 8 heads]       += V^T [D x 16] P^T        (V by ldmatrix.trans)
+//
+// S^T's result layout turns into P^T's operand layout by one 8x8 transpose
+// (movmatrix), and the heads of S^T, P^T and O^T lie in the same lanes, so
+// maxima and rescales need no exchange. G up to 16 heads take one or two
+// tiles of 8; more take several passes over K and V.
+//
+// P enters the second product as the sum of two values of the input type (high
+// part and remainder), so that the weights keep 16 bits and more: the
+// tensor pipe has the room, and the output is then rounded once, as the formula is.
+//
+// Split: the 16-key blocks of all (sequence, kv head) items, in order, are cut
+// into equal ranges, one per CTA, whatever the lengths: the last CTA ends when the
+// first does. A CTA joins its 8 warps in shared memory; an item cut by a range
+// end leaves fp32 partials (O, maximum, sum) in the workspace, and the CTA
+// that counts the last of its parts joins them, in the order of the parts.
+
+#include <string.h>
 
 #include "ragged.cuh"
 
@@ -9,74 +40,470 @@ namespace afd {
 
 namespace {
 
-// One CTA of 8 warps per (sequence, head): the warps take every eighth key,
-// each with its own running maximum and sum, and join at the end.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_decode_kernel(PagedDecodeArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int E = D / 32;
-  __shared__ float om[8][D], mm[8], ll[8];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int b = blockIdx.x / a.nq, h = blockIdx.x % a.nq, kvh = h / (a.nq / a.nkv);
-  const T* q = reinterpret_cast<const T*>(a.q) + (size_t)b * a.q_row + (size_t)h * D;
-  const int len = checked_len(a.seq_lens[b], a.max_pages * a.page_size, a.status, 221);
-  float qv[E], o[E];
-  for (int i = 0; i < E; ++i) {
-    qv[i] = to_f(q[lane * E + i]) * a.scale;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = warp; j < len; j += 8) {
-    const int page = a.page_table[(size_t)b * a.table_row + j / a.page_size];
-    const bool ok = page >= 0 && page < a.num_pages;
-    if (!ok) report_status(a.status, kBoundsViolation, 222);
-    const size_t at = (size_t)(ok ? page : 0) * a.page_stride +
-                      ((size_t)kvh * a.page_size + j % a.page_size) * D;
-    const T* k = reinterpret_cast<const T*>(a.k_pages) + at;
-    const T* v = reinterpret_cast<const T*>(a.v_pages) + at;
-    float s = 0.f;
-    for (int i = 0; i < E; ++i) s += qv[i] * (ok ? to_f(k[lane * E + i]) : 0.f);
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float m_new = fmaxf(m, s);
-    const float c = m_new == -INFINITY ? 1.f : __expf(m - m_new);
-    const float p = m_new == -INFINITY ? 0.f : __expf(s - m_new);
-    l = l * c + p;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * c + p * (ok ? to_f(v[lane * E + i]) : 0.f);
-    m = m_new;
-  }
-  for (int i = 0; i < E; ++i) om[warp][lane * E + i] = o[i];
-  if (lane == 0) {
-    mm[warp] = m;
-    ll[warp] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, mm[w]);
-    for (int w = 0; w < 8; ++w) {
-      const float c = mm[w] == -INFINITY ? 0.f : __expf(mm[w] - M);
-      L += ll[w] * c;
-      acc += om[w][threadIdx.x] * c;
-    }
-    T* out = reinterpret_cast<T*>(a.out) + ((size_t)b * a.nq + h) * D;
-    out[threadIdx.x] = from_f<T>(L > 0.f ? acc / L : 0.f);
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kBlk = 16;                 // keys of a block
+constexpr int kStages = 3;               // ring depth of a warp
+constexpr int kMinBlocks = 4 * kWarps;   // blocks of a CTA's range at least
+
+template <int D>
+struct Dec {
+  static constexpr int kBox = kBlk * 128;             // one 128-byte wide box
+  static constexpr int kTile = kBlk * D * 2;          // K or V of a block
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kJoin = kWarps * 8 * D * 4;
+  static constexpr int kBytes = kRing + kJoin + 1024 /*align*/ + 1536 /*barriers, statistics*/;
+};
+
+// Float index of (warp, head, dim) in the join buffer: the heads of a quarter
+// warp start 8 banks apart.
+template <int D>
+__device__ __forceinline__ int join_at(int w, int h, int d) {
+  return (w * 8 + h) * D + (d ^ ((h >> 1) * 8));
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    mma_16816_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
 
+// Position in the order of all blocks: item (sequence b, kv head and head group
+// `sub`), the item's first block and its end.
+struct Cursor {
+  int b, sub, len;
+  long long begin, end;
+};
+
 }  // namespace
 
-int launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t s) {
-  if (a.B == 0) return 0;
-  const dim3 grid((unsigned)(a.B * a.nq));
-  cudaError_t e;
-  if (a.elem == kElemBf16)
-    e = a.D == 128 ? launch_k(paged_decode_kernel<__nv_bfloat16, 128>, grid, dim3(256), 0, s, a)
-                   : launch_k(paged_decode_kernel<__nv_bfloat16, 64>, grid, dim3(256), 0, s, a);
-  else
-    e = a.D == 128 ? launch_k(paged_decode_kernel<__half, 128>, grid, dim3(256), 0, s, a)
-                   : launch_k(paged_decode_kernel<__half, 64>, grid, dim3(256), 0, s, a);
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap tk,
+                        const __grid_constant__ CUtensorMap tv, PagedDecodeArgs a, int groups) {
+  using C = Dec<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* join = reinterpret_cast<float*>(smem + C::kRing);           // [warps][8][D], join_at
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kJoin);  // [warps][stages]
+  float2* ml = reinterpret_cast<float2*>(full + kWarps * kStages);   // [2][warps][8]
+  long long* scan = reinterpret_cast<long long*>(ml + 2 * kWarps * 8);  // [warps]
+  Cursor* first = reinterpret_cast<Cursor*>(scan + kWarps);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(first + 1);
+  volatile int* last_part = abort_flag + 1;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int G = a.nq / a.nkv, subs = a.nkv * groups;
+  const int most = a.max_pages * a.page_size;
+  if (threadIdx.x < kWarps * kStages) mbar_init(&full[threadIdx.x], 1);
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    first->b = a.B;
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  fence_barrier_init();
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's range of blocks: a scan over the sequences' block counts
+  const int chunk = (a.B + kThreads - 1) / kThreads;
+  const int b0 = min(a.B, (int)threadIdx.x * chunk), b1 = min(a.B, b0 + chunk);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int len = checked_len(a.seq_lens[b], most, a.status, 221);
+    mine += (long long)((len + kBlk - 1) / kBlk) * subs;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  long long total = 0, before = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = total;
+    total += scan[w];
+  }
+  before += upto - mine;
+  long long range = (total + gridDim.x - 1) / gridDim.x;
+  range = max((long long)kMinBlocks, (range + kWarps - 1) / kWarps * kWarps);
+  const long long r0 = min(total, (long long)blockIdx.x * range), r1 = min(total, r0 + range);
+  if (r0 < r1 && before <= r0 && r0 < before + mine) {
+    long long at = before;
+    for (int b = b0; b < b1; ++b) {
+      const int len = checked_len(a.seq_lens[b], most, nullptr, 0);
+      const long long blocks = (len + kBlk - 1) / kBlk;
+      if (r0 < at + blocks * subs) {
+        first->b = b;
+        first->len = len;
+        first->sub = (int)((r0 - at) / blocks);
+        first->begin = at + first->sub * blocks;
+        first->end = first->begin + blocks;
+        break;
+      }
+      at += blocks * subs;
+    }
+  }
+  // sequences without a key: zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
+      for (int i = threadIdx.x; i < a.nq * D / 8; i += kThreads)
+        reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (size_t)b * a.nq * D)[i] =
+            make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  if (r0 >= r1) return;
+
+  auto next_item = [&](Cursor& c) {
+    c.begin = c.end;
+    if (++c.sub == subs) {
+      c.sub = 0;
+      do {
+        ++c.b;
+        c.len = c.b < a.B ? checked_len(a.seq_lens[c.b], most, nullptr, 0) : 1;
+      } while (c.len == 0);
+    }
+    c.end = c.begin + (c.len + kBlk - 1) / kBlk;
+  };
+
+  // ---- the warp's loads: blocks r0 + warp, r0 + warp + 8, ... of the range
+  uint8_t* ring = smem + warp * kStages * C::kStage;
+  uint64_t* bar = full + warp * kStages;
+  Cursor ic = *first;
+  long long issue_at = r0 + warp;
+  int issued = 0, page = 0;
+  auto look_up = [&]() {  // the page of the next block to load
+    if (issue_at >= r1) return;
+    while (issue_at >= ic.end) next_item(ic);
+    page = a.page_table[(size_t)ic.b * a.table_row +
+                        (int)((issue_at - ic.begin) * kBlk / a.page_size)];
+  };
+  auto issue = [&]() {
+    if (issue_at >= r1) return;
+    const int st = issued % kStages;
+    if (lane == 0) {
+      if (page < 0 || page >= a.num_pages)  // the copies fill with zeros
+        report_status(a.status, kBoundsViolation, 222);
+      const int row = (ic.sub / groups) * a.page_size +
+                      (int)((issue_at - ic.begin) * kBlk % a.page_size);
+      uint8_t* dst = ring + st * C::kStage;
+      mbar_arrive_expect_tx(&bar[st], C::kStage);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load_3d(dst + c * C::kBox, &tk, &bar[st], c * 64, row, page);
+        tma_load_3d(dst + C::kTile + c * C::kBox, &tv, &bar[st], c * 64, row, page);
+      }
+    }
+    ++issued;
+    issue_at += kWarps;
+    look_up();
+  };
+  look_up();
+  for (int s = 0; s < kStages; ++s) issue();
+
+  // ---- the items of the range
+  const float scale_log2 = a.scale * 1.4426950408889634f;
+  Cursor cc = *first;
+  long long at = r0 + warp;
+  int used = 0, joins = 0;
+  bool ok = true;
+  for (;; next_item(cc)) {
+    const int kvh = cc.sub / groups, grp = cc.sub % groups;
+    const int h0 = kvh * G + grp * 8 * NT;                 // first query head of the item
+    const int heads = min(8 * NT, G - grp * 8 * NT);
+    const long long end = min(cc.end, r1);
+    // Q^T as the B operand: head lane / 4, dims 2 (lane % 4) + {0, 1, 8, 9} of 16
+    uint32_t qf[NT][D / 16][2];
+    const T* q = reinterpret_cast<const T*>(a.q) + (size_t)cc.b * a.q_row + (size_t)h0 * D;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qf[n][kk][e] = n * 8 + lane / 4 < heads
+                             ? *reinterpret_cast<const uint32_t*>(
+                                   q + (n * 8 + lane / 4) * D + kk * 16 + (lane % 4) * 2 + e * 8)
+                             : 0u;
+    // lane: heads 2 (lane % 4) + {0, 1} of each tile
+    float m[NT][2], l[NT][2], o[NT][D / 16][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
+    }
+    for (; at < end; at += kWarps) {
+      const int st = used % kStages;
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(&bar[st], (used / kStages) & 1, abort_flag,
+                                                   a.status, 223)))
+        ok = false;
+      const uint32_t ks = smem_u32(ring + st * C::kStage), vs = ks + C::kTile;
+      const int key0 = (int)(at - cc.begin) * kBlk;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      {
+        const int r = (lane / 8 % 2) * 8 + lane % 8;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kf[4];
+          const int ch = (kk % 4) * 2 + lane / 16;
+          ldsm4(ks + (kk / 4) * C::kBox + r * 128 + ((ch ^ (r & 7)) << 4), kf);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<T>(s[n], kf, qf[n][kk][0], qf[n][kk][1]);
+        }
+      }
+      if (key0 + kBlk > cc.len) {
+        // keys past the end: no weight, and finite values for it to meet
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + lane / 4 + (e / 2) * 8 >= cc.len) s[n][e] = -INFINITY;
+        for (int i = lane; i < kBlk * D / 8; i += 32) {
+          const int r = i / 8 % kBlk;
+          if (key0 + r >= cc.len)
+            *reinterpret_cast<uint4*>(ring + st * C::kStage + C::kTile + i * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = s[n][e] * scale_log2;
+        // the maximum moves only when it grows by more than 8 (powers of two)
+        const bool grow = fmaxf(x[0], x[2]) > m[n][0] + 8.f || fmaxf(x[1], x[3]) > m[n][1] + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(m[n][e], fmaxf(x[e], x[e + 2]));
+#pragma unroll
+            for (int f = 4; f < 32; f <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, f));
+            const float c = mx == -INFINITY ? 1.f : exp2_approx(m[n][e] - mx);
+            m[n][e] = mx;
+            l[n][e] *= c;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[n][d][e] *= c;
+              o[n][d][e + 2] *= c;
+            }
+          }
+        }
+        float p[4], r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = m[n][e & 1] == -INFINITY ? 0.f : exp2_approx(x[e] - m[n][e & 1]);
+          r[e] = p[e] - to_f(from_f<T>(p[e]));
+        }
+        l[n][0] += p[0] + p[2];
+        l[n][1] += p[1] + p[3];
+        ph[n][0] = transpose8(pack2<T>(p[0], p[1]));
+        ph[n][1] = transpose8(pack2<T>(p[2], p[3]));
+        pl[n][0] = transpose8(pack2<T>(r[0], r[1]));
+        pl[n][1] = transpose8(pack2<T>(r[2], r[3]));
+      }
+      {
+        const int r = (lane / 16) * 8 + lane % 8;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          uint32_t vf[4];
+          const int ch = (d % 4) * 2 + (lane / 8) % 2;
+          ldsm4_t(vs + (d / 4) * C::kBox + r * 128 + ((ch ^ (r & 7)) << 4), vf);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816<T>(o[n][d], vf, ph[n][0], ph[n][1]);
+            mma16816<T>(o[n][d], vf, pl[n][0], pl[n][1]);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the block
+      ++used;
+      issue();
+    }
+
+    // ---- join the warps; a cut item leaves a part, the last of which joins them
+    const bool cut = cc.begin < r0 || cc.end > r1;
+    const int c0 = (int)(cc.begin / range), parts = (int)((cc.end - 1) / range) - c0 + 1;
+    const int slot = cc.begin < r0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
+#pragma unroll
+    for (int n = 0; n < NT; ++n, ++joins) {
+      float2* mls = ml + (joins & 1) * kWarps * 8;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int f = 4; f < 32; f <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], f);
+        if (lane < 4) mls[warp * 8 + lane * 2 + e] = make_float2(m[n][e], l[n][e]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = (lane % 4) * 2 + e;
+        float M = -INFINITY;
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mls[w * 8 + h].x);
+        const float c = m[n][e] == -INFINITY ? 0.f : exp2_approx(m[n][e] - M);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          join[join_at<D>(warp, h, d * 16 + lane / 4)] = o[n][d][e] * c;
+          join[join_at<D>(warp, h, d * 16 + 8 + lane / 4)] = o[n][d][e + 2] * c;
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 8 * D / 4; i += kThreads) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4, head = n * 8 + h;
+        if (head >= heads) break;
+        float M = -INFINITY, lsum = 0.f;
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mls[w * 8 + h].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 s = mls[w * 8 + h];
+          lsum += s.x == -INFINITY ? 0.f : s.y * exp2_approx(s.x - M);
+          const float4 v = *reinterpret_cast<const float4*>(join + join_at<D>(w, h, d));
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
+        }
+        if (cut) {
+          const size_t at_part = (size_t)slot * 8 * NT + head;
+          *reinterpret_cast<float4*>(a.o_part + at_part * D + d) = acc;
+          if (d == 0) a.ml_part[at_part] = make_float2(M, lsum);
+        } else {
+          const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+          uint2 v = make_uint2(0u, 0u);
+          if (lsum > 0.f || lsum != lsum)
+            v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) +
+                                    ((size_t)cc.b * a.nq + h0 + head) * D + d) = v;
+        }
+      }
+    }
+    if (cut) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) *last_part = atomicAdd(&a.counters[c0], 1) == parts - 1;
+      __syncthreads();
+      if (*last_part) {
+        __threadfence();
+        for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
+          const int head = i / (D / 4), d = i % (D / 4) * 4;
+          auto part = [&](int p) {
+            return (size_t)(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * 8 * NT + head;
+          };
+          float M = -INFINITY, lsum = 0.f;
+#pragma unroll 4
+          for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(&a.ml_part[part(p)]).x);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int p = 0; p < parts; ++p) {
+            const float2 s = __ldcg(&a.ml_part[part(p)]);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.o_part + part(p) * D + d));
+            const float c = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
+            lsum += s.y * c;
+            acc.x += v.x * c;
+            acc.y += v.y * c;
+            acc.z += v.z * c;
+            acc.w += v.w * c;
+          }
+          const float inv = 1.f / lsum;
+          uint2 v = make_uint2(0u, 0u);
+          if (lsum > 0.f || lsum != lsum)
+            v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) +
+                                    ((size_t)cc.b * a.nq + h0 + head) * D + d) = v;
+        }
+        if (threadIdx.x == 0) a.counters[c0] = 0;
+      }
+      __syncthreads();  // last_part is written again at the next cut
+    }
+    if (cc.end >= r1) break;
+  }
+  if (!ok && lane == 0) {
+    // loads that a failed wait left in flight must land before the CTA exits
+    volatile int no_abort = 0;
+    for (int j = max(0, issued - kStages); j < issued; ++j)
+      mbar_wait(&bar[j % kStages], (j / kStages) & 1, &no_abort, nullptr, 224, 100000000ull);
+  }
+}
+
+// ============================================================ host side ===
+
+template <typename T, int D, int NT>
+static int launch_one(const PagedDecodeArgs& a, int grid, int groups, const CUtensorMap& tk,
+                      const CUtensorMap& tv, cudaStream_t s) {
+  const auto kern = paged_decode_kernel<T, D, NT>;
+  cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), Dec<D>::kBytes);
+  if (e == cudaSuccess)
+    e = launch_k(kern, dim3(grid), dim3(kThreads), Dec<D>::kBytes, s, tk, tv, a, groups);
   return e == cudaSuccess ? 0 : 4000 + (int)e;
+}
+
+long long paged_decode_part_rows(int nq, int nkv, int grid) {
+  return 2ll * grid * (nq / nkv > 8 ? 16 : 8);
+}
+
+int launch_paged_decode(const PagedDecodeArgs& a, int grid, cudaStream_t s) {
+  if (a.B == 0) return 0;
+  CUtensorMap tk, tv;
+  // pool [pages, nkv * page_size, D]: a box is the 16 rows of a block
+  const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.nkv * a.page_size, (uint64_t)a.num_pages};
+  const uint64_t str[2] = {(uint64_t)a.D * 2, (uint64_t)a.page_stride * 2};
+  const uint32_t box[3] = {64, kBlk, 1};
+  if (int e = encode_map16(&tk, a.k_pages, a.elem, 3, dims, str, box)) return e;
+  if (int e = encode_map16(&tv, a.v_pages, a.elem, 3, dims, str, box)) return e;
+  const int G = a.nq / a.nkv, groups = (G + 15) / 16;
+#define AFD_DECODE(T, D)                                            \
+  (G > 8 ? launch_one<T, D, 2>(a, grid, groups, tk, tv, s)          \
+         : launch_one<T, D, 1>(a, grid, groups, tk, tv, s))
+  if (a.elem == kElemBf16)
+    return a.D == 128 ? AFD_DECODE(__nv_bfloat16, 128) : AFD_DECODE(__nv_bfloat16, 64);
+  return a.D == 128 ? AFD_DECODE(__half, 128) : AFD_DECODE(__half, 64);
+#undef AFD_DECODE
 }
 
 }  // namespace afd

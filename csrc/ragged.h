@@ -34,11 +34,16 @@ struct PagedDecodeArgs {
   const int* seq_lens;      // [B]
   void* out;                // [B, nq, D]
   int B, nq, nkv, D, num_pages, page_size, max_pages;
-  float scale;
+  float scale;              // > 0
   int elem;
   int* status;              // optional [2]
+  float* o_part;            // [paged_decode_part_rows, D]
+  float2* ml_part;          // [paged_decode_part_rows]
+  int* counters;            // [grid], zero; left zero
 };
-int launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t s);
+// Rows of the workspace of a launch with `grid` CTAs.
+long long paged_decode_part_rows(int nq, int nkv, int grid);
+int launch_paged_decode(const PagedDecodeArgs& a, int grid, cudaStream_t s);
 
 // Causal attention of packed queries. Sequence i owns query rows
 // cu_q[i] .. cu_q[i+1] - 1; they are its last positions. Keys and values come
