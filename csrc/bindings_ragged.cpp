@@ -171,6 +171,9 @@ at::Tensor paged_decode_attention(const at::Tensor& q_in, const at::Tensor& k_pa
   a.scale = scale_of(scale, a.D);
   a.status = status_ptr(status, q);
   const int grid = num_sms();
+  TORCH_CHECK_VALUE((double)a.B * (a.max_pages * (a.page_size / 16.0) + 4) * a.nkv *
+                            ((a.nq / a.nkv + 15) / 16) < 2147483648.0 - 4096.0 * grid,
+                    "the page table spans too many positions in all");
   const int64_t parts = paged_decode_part_rows(a.nq, a.nkv, grid);
   const at::Tensor ws = at::empty({parts * (a.D + 2)}, q.options().dtype(at::kFloat));
   const at::Tensor counters = zeroed_counters(q, grid);

@@ -44,7 +44,16 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlk = 16;                 // keys of a block
 constexpr int kStages = 3;               // ring depth of a warp
-constexpr int kMinBlocks = 4 * kWarps;   // blocks of a CTA's range at least
+// Units of a range: blocks, and kItemCost more for an item (its queries, the
+// join of the warps: about what the HBM delivers of 4 blocks to an SM). A range
+// holds at least kMinRange of them, so that short sequences stay whole. A range
+// end near an item's end is moved there, within half a range where ranges are
+// short (up to kShortRange) and within kSnap units where they are long: a cut
+// costs a join through the workspace, an uneven range what it has more.
+constexpr int kItemCost = 4;
+constexpr int kMinRange = 20;
+constexpr int kShortRange = 40;
+constexpr int kSnap = 8;
 
 template <int D>
 struct Dec {
@@ -103,11 +112,31 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
   }
 }
 
-// Position in the order of all blocks: item (sequence b, kv head and head group
-// `sub`), the item's first block and its end.
+// Four output values of a head, from their weighted sum and the weights' sum.
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const PagedDecodeArgs& a, int b, int h, int d, float4 acc,
+                                          float l) {
+  const float inv = 1.f / l;
+  uint2 v = make_uint2(0u, 0u);  // every weight 0
+  if (!(l == 0.f))
+    v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + ((size_t)b * a.nq + h) * D + d) = v;
+}
+
+// A place in the order of all work: item (sequence b, kv head and head group
+// `sub`), the item's extent [begin, end) in units of blocks, kItemCost of them
+// for the item itself, and the portion [j0, j1) of its blocks that is this CTA's.
+// `before` counts the CTA's blocks of earlier items: block j goes to warp
+// (before + j - j0) % kWarps.
 struct Cursor {
+  int b, sub, len, len_next;
+  int begin, end;
+  int j0, j1, before;
+};
+
+struct Place {  // of a range end: the item that it falls into, moved to an end of it if near
   int b, sub, len;
-  long long begin, end;
+  int begin, end, at;
 };
 
 }  // namespace
@@ -122,11 +151,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* join = reinterpret_cast<float*>(smem + C::kRing);           // [warps][8][D], join_at
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kJoin);  // [warps][stages]
-  float2* ml = reinterpret_cast<float2*>(full + kWarps * kStages);   // [2][warps][8]
-  long long* scan = reinterpret_cast<long long*>(ml + 2 * kWarps * 8);  // [warps]
-  Cursor* first = reinterpret_cast<Cursor*>(scan + kWarps);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(first + 1);
-  volatile int* last_part = abort_flag + 1;
+  float2* ml = reinterpret_cast<float2*>(full + kWarps * kStages);   // [warps][8]
+  int* scan = reinterpret_cast<int*>(ml + kWarps * 8);               // [warps]
+  Place* place = reinterpret_cast<Place*>(scan + kWarps);            // [2]: of r0, r1
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(place + 2);
+  volatile int* joins_item = abort_flag + 1;                         // [2]
+  volatile int* any_empty = joins_item + 2;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = a.nq / a.nkv, subs = a.nkv * groups;
@@ -134,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x < kWarps * kStages) mbar_init(&full[threadIdx.x], 1);
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    first->b = a.B;
+    *any_empty = 0;
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
@@ -142,117 +172,169 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's range of blocks: a scan over the sequences' block counts
+  // ---- this CTA's range of the work: a scan over the sequences' extents
+  auto extent = [](int len) { return len > 0 ? (len + kBlk - 1) / kBlk + kItemCost : 0; };
   const int chunk = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * chunk), b1 = min(a.B, b0 + chunk);
-  long long mine = 0;
+  int mine = 0;
+  bool empty = false;
   for (int b = b0; b < b1; ++b) {
     const int len = checked_len(a.seq_lens[b], most, a.status, 221);
-    mine += (long long)((len + kBlk - 1) / kBlk) * subs;
+    mine += extent(len) * subs;
+    empty |= len == 0 && b % gridDim.x == blockIdx.x;
   }
-  long long upto = mine;
+  int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
-  long long total = 0, before = 0;
+  if (empty) *any_empty = 1;
+  int total = 0, before = 0;
   for (int w = 0; w < kWarps; ++w) {
     if (w == warp) before = total;
     total += scan[w];
   }
   before += upto - mine;
-  long long range = (total + gridDim.x - 1) / gridDim.x;
-  range = max((long long)kMinBlocks, (range + kWarps - 1) / kWarps * kWarps);
-  const long long r0 = min(total, (long long)blockIdx.x * range), r1 = min(total, r0 + range);
-  if (r0 < r1 && before <= r0 && r0 < before + mine) {
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int len = checked_len(a.seq_lens[b], most, nullptr, 0);
-      const long long blocks = (len + kBlk - 1) / kBlk;
-      if (r0 < at + blocks * subs) {
-        first->b = b;
-        first->len = len;
-        first->sub = (int)((r0 - at) / blocks);
-        first->begin = at + first->sub * blocks;
-        first->end = first->begin + blocks;
-        break;
+  const int range = max(kMinRange, (int)((total + gridDim.x - 1) / gridDim.x));
+  // a range end this near to an item's is moved there
+  const int snap = range <= kShortRange ? range / 2 : kSnap;
+  const bool works = (long long)blockIdx.x * range < total;
+  const int raw0 = works ? blockIdx.x * range : total;
+  if (works) {
+    for (int e = 0; e < 2; ++e) {
+      const int r = raw0 + e * range;
+      if (r < before || r - before >= mine) continue;
+      int at = before;
+      for (int b = b0; b < b1; ++b) {
+        const int len = checked_len(a.seq_lens[b], most, nullptr, 0);
+        const int ext = extent(len);
+        if (r - at < ext * subs) {
+          Place p;
+          p.b = b;
+          p.len = len;
+          p.sub = (r - at) / ext;
+          p.begin = at + p.sub * ext;
+          p.end = p.begin + ext;
+          p.at = r - p.begin <= snap ? p.begin : p.end - r <= snap ? p.end : r;
+          place[e] = p;
+          break;
+        }
+        at += ext * subs;
       }
-      at += blocks * subs;
     }
   }
-  // sequences without a key: zeros
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
-      for (int i = threadIdx.x; i < a.nq * D / 8; i += kThreads)
-        reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (size_t)b * a.nq * D)[i] =
-            make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0 && total - raw0 <= range) place[1].at = total;
   __syncthreads();
-  if (r0 >= r1) return;
+  const int r0 = works ? place[0].at : total, r1 = place[1].at;
 
+  // the item after `c` and this CTA's portion of it
+  auto take = [&](Cursor& c) {
+    c.j0 = r0 > c.begin ? r0 - c.begin - kItemCost : 0;
+    c.j1 = min(c.end, r1) - c.begin - kItemCost;
+  };
   auto next_item = [&](Cursor& c) {
+    c.before += c.j1 - c.j0;
     c.begin = c.end;
     if (++c.sub == subs) {
       c.sub = 0;
       do {
         ++c.b;
-        c.len = c.b < a.B ? checked_len(a.seq_lens[c.b], most, nullptr, 0) : 1;
+        c.len = c.b < a.B ? checked_len(c.len_next, most, nullptr, 0) : 1;
+        c.len_next = c.b + 1 < a.B ? a.seq_lens[c.b + 1] : 0;
       } while (c.len == 0);
     }
-    c.end = c.begin + (c.len + kBlk - 1) / kBlk;
+    c.end = c.begin + extent(c.len);
+    take(c);
   };
+  Cursor ic;
+  if (r0 < r1) {
+    const Place p = place[0];
+    ic.b = p.b;
+    ic.sub = p.sub;
+    ic.len = p.len;
+    ic.len_next = p.b + 1 < a.B ? a.seq_lens[p.b + 1] : 0;
+    ic.begin = p.begin;
+    ic.end = p.end;
+    ic.before = 0;
+    if (r0 == p.end) {
+      ic.j0 = ic.j1 = 0;
+      next_item(ic);
+    } else {
+      take(ic);
+    }
+  }
+  Cursor cc = ic;
 
-  // ---- the warp's loads: blocks r0 + warp, r0 + warp + 8, ... of the range
+  // ---- the warp's loads, kStages blocks ahead
   uint8_t* ring = smem + warp * kStages * C::kStage;
   uint64_t* bar = full + warp * kStages;
-  Cursor ic = *first;
-  long long issue_at = r0 + warp;
-  int issued = 0, page = 0;
-  auto look_up = [&]() {  // the page of the next block to load
-    if (issue_at >= r1) return;
-    while (issue_at >= ic.end) next_item(ic);
-    page = a.page_table[(size_t)ic.b * a.table_row +
-                        (int)((issue_at - ic.begin) * kBlk / a.page_size)];
+  auto first_block = [&](const Cursor& c) { return c.j0 + ((warp - c.before) & (kWarps - 1)); };
+  int issued = 0, ij = 0, held = 0, page = 0, row = 0;
+  bool more = r0 < r1;
+  // each lane holds the page of one of the next 32 blocks
+  auto look_up = [&]() {
+    const int key = (ij + lane * kWarps) * kBlk;
+    held = 0;
+    if (more && key < ic.j1 * kBlk) {
+      page = a.page_table[(size_t)ic.b * a.table_row + key / a.page_size];
+      row = (ic.sub / groups) * a.page_size + key % a.page_size;
+    }
+  };
+  auto find = [&]() {  // the item of the next block to load
+    while (more && ij >= ic.j1) {
+      if (ic.end >= r1) {
+        more = false;
+      } else {
+        next_item(ic);
+        ij = first_block(ic);
+      }
+    }
+    look_up();
   };
   auto issue = [&]() {
-    if (issue_at >= r1) return;
+    if (!more) return;
     const int st = issued % kStages;
+    const int pg = __shfl_sync(0xffffffffu, page, held), rw = __shfl_sync(0xffffffffu, row, held);
     if (lane == 0) {
-      if (page < 0 || page >= a.num_pages)  // the copies fill with zeros
+      if (pg < 0 || pg >= a.num_pages)  // the copies fill with zeros
         report_status(a.status, kBoundsViolation, 222);
-      const int row = (ic.sub / groups) * a.page_size +
-                      (int)((issue_at - ic.begin) * kBlk % a.page_size);
       uint8_t* dst = ring + st * C::kStage;
       mbar_arrive_expect_tx(&bar[st], C::kStage);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        tma_load_3d(dst + c * C::kBox, &tk, &bar[st], c * 64, row, page);
-        tma_load_3d(dst + C::kTile + c * C::kBox, &tv, &bar[st], c * 64, row, page);
+        tma_load_3d(dst + c * C::kBox, &tk, &bar[st], c * 64, rw, pg);
+        tma_load_3d(dst + C::kTile + c * C::kBox, &tv, &bar[st], c * 64, rw, pg);
       }
     }
     ++issued;
-    issue_at += kWarps;
-    look_up();
+    ij += kWarps;
+    if (ij >= ic.j1)
+      find();
+    else if (++held == 32)
+      look_up();
   };
-  look_up();
+  if (more) ij = first_block(ic);
+  find();
   for (int s = 0; s < kStages; ++s) issue();
 
-  // ---- the items of the range
-  const float scale_log2 = a.scale * 1.4426950408889634f;
-  Cursor cc = *first;
-  long long at = r0 + warp;
-  int used = 0, joins = 0;
-  bool ok = true;
-  for (;; next_item(cc)) {
-    const int kvh = cc.sub / groups, grp = cc.sub % groups;
-    const int h0 = kvh * G + grp * 8 * NT;                 // first query head of the item
+  // sequences without a key: zeros
+  if (*any_empty)
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
+        for (int i = threadIdx.x; i < a.nq * D / 8; i += kThreads)
+          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (size_t)b * a.nq * D)[i] =
+              make_uint4(0, 0, 0, 0);
+  if (r0 >= r1) return;
+
+  // Q^T as the B operand: head lane / 4, dims 2 (lane % 4) + {0, 1, 8, 9} of 16
+  uint32_t qf[NT][D / 16][2];
+  auto load_q = [&](const Cursor& c) {
+    const int grp = c.sub % groups, h0 = (c.sub / groups) * G + grp * 8 * NT;
     const int heads = min(8 * NT, G - grp * 8 * NT);
-    const long long end = min(cc.end, r1);
-    // Q^T as the B operand: head lane / 4, dims 2 (lane % 4) + {0, 1, 8, 9} of 16
-    uint32_t qf[NT][D / 16][2];
-    const T* q = reinterpret_cast<const T*>(a.q) + (size_t)cc.b * a.q_row + (size_t)h0 * D;
+    const T* q = reinterpret_cast<const T*>(a.q) + (size_t)c.b * a.q_row + (size_t)h0 * D;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -263,6 +345,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                              ? *reinterpret_cast<const uint32_t*>(
                                    q + (n * 8 + lane / 4) * D + kk * 16 + (lane % 4) * 2 + e * 8)
                              : 0u;
+  };
+  load_q(cc);
+
+  // The cuts of an item lie at the multiples of `range` inside it that are not
+  // near its ends: CTA `first` has its first part, CTA first + p its part p.
+  auto first_cta = [&](int begin) { return (begin + snap) / range; };
+  auto parts_of = [&](int begin, int end) { return (end - snap - 1) / range - first_cta(begin) + 1; };
+  auto part_row = [&](int c0, int p) { return (size_t)(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * 8 * NT; };
+
+  // ---- the items of the range
+  const float scale_log2 = a.scale * 1.4426950408889634f;
+  const Cursor head = cc;
+  int used = 0;
+  bool ok = true;
+  for (;;) {
+    const int grp = cc.sub % groups, h0 = (cc.sub / groups) * G + grp * 8 * NT;
+    const int heads = min(8 * NT, G - grp * 8 * NT);
     // lane: heads 2 (lane % 4) + {0, 1} of each tile
     float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
@@ -274,13 +373,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
     }
-    for (; at < end; at += kWarps) {
+    for (int j = first_block(cc); j < cc.j1; j += kWarps) {
       const int st = used % kStages;
       if (ok && !__all_sync(0xffffffffu, mbar_wait(&bar[st], (used / kStages) & 1, abort_flag,
                                                    a.status, 223)))
         ok = false;
       const uint32_t ks = smem_u32(ring + st * C::kStage), vs = ks + C::kTile;
-      const int key0 = (int)(at - cc.begin) * kBlk;
+      const int key0 = j * kBlk;
       float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -367,101 +466,111 @@ __global__ void __launch_bounds__(kThreads, 1)
       issue();
     }
 
-    // ---- join the warps; a cut item leaves a part, the last of which joins them
-    const bool cut = cc.begin < r0 || cc.end > r1;
-    const int c0 = (int)(cc.begin / range), parts = (int)((cc.end - 1) / range) - c0 + 1;
-    const int slot = cc.begin < r0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
+    // ---- join the warps; the next item's queries are on their way meanwhile
+    const Cursor item = cc;
+    const bool more_items = cc.end < r1;
+    if (more_items) {
+      next_item(cc);
+      load_q(cc);
+    }
+    const bool cut = item.begin < r0 || item.end > r1;
+    const size_t row0 = (size_t)(item.begin < r0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1) * 8 * NT;
 #pragma unroll
-    for (int n = 0; n < NT; ++n, ++joins) {
-      float2* mls = ml + (joins & 1) * kWarps * 8;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int f = 4; f < 32; f <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], f);
-        if (lane < 4) mls[warp * 8 + lane * 2 + e] = make_float2(m[n][e], l[n][e]);
-      }
-      __syncthreads();
+    for (int n = 0; n < NT; ++n) {
+      __syncthreads();  // the buffer's last readers are done
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = (lane % 4) * 2 + e;
-        float M = -INFINITY;
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mls[w * 8 + h].x);
-        const float c = m[n][e] == -INFINITY ? 0.f : exp2_approx(m[n][e] - M);
+#pragma unroll
+        for (int f = 4; f < 32; f <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], f);
+        if (lane < 4) ml[warp * 8 + h] = make_float2(m[n][e], l[n][e]);
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-          join[join_at<D>(warp, h, d * 16 + lane / 4)] = o[n][d][e] * c;
-          join[join_at<D>(warp, h, d * 16 + 8 + lane / 4)] = o[n][d][e + 2] * c;
+          join[join_at<D>(warp, h, d * 16 + lane / 4)] = o[n][d][e];
+          join[join_at<D>(warp, h, d * 16 + 8 + lane / 4)] = o[n][d][e + 2];
         }
       }
       __syncthreads();
       for (int i = threadIdx.x; i < 8 * D / 4; i += kThreads) {
-        const int h = i / (D / 4), d = i % (D / 4) * 4, head = n * 8 + h;
-        if (head >= heads) break;
+        const int h = i / (D / 4), d = i % (D / 4) * 4, hd = n * 8 + h;
+        if (hd >= heads) break;
         float M = -INFINITY, lsum = 0.f;
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mls[w * 8 + h].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w * 8 + h].x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float2 s = mls[w * 8 + h];
-          lsum += s.x == -INFINITY ? 0.f : s.y * exp2_approx(s.x - M);
+          const float2 s = ml[w * 8 + h];
+          const float c = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
           const float4 v = *reinterpret_cast<const float4*>(join + join_at<D>(w, h, d));
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
+          lsum += s.y * c;
+          acc.x += v.x * c;
+          acc.y += v.y * c;
+          acc.z += v.z * c;
+          acc.w += v.w * c;
         }
         if (cut) {
-          const size_t at_part = (size_t)slot * 8 * NT + head;
-          *reinterpret_cast<float4*>(a.o_part + at_part * D + d) = acc;
-          if (d == 0) a.ml_part[at_part] = make_float2(M, lsum);
+          *reinterpret_cast<float4*>(a.o_part + (row0 + hd) * D + d) = acc;
+          if (d == 0) a.ml_part[row0 + hd] = make_float2(M, lsum);
         } else {
-          const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-          uint2 v = make_uint2(0u, 0u);
-          if (lsum > 0.f || lsum != lsum)
-            v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) +
-                                    ((size_t)cc.b * a.nq + h0 + head) * D + d) = v;
+          store_out<T, D>(a, item.b, h0 + hd, d, acc, lsum);
         }
       }
     }
-    if (cut) {
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) *last_part = atomicAdd(&a.counters[c0], 1) == parts - 1;
-      __syncthreads();
-      if (*last_part) {
-        __threadfence();
-        for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
-          const int head = i / (D / 4), d = i % (D / 4) * 4;
-          auto part = [&](int p) {
-            return (size_t)(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * 8 * NT + head;
-          };
-          float M = -INFINITY, lsum = 0.f;
-#pragma unroll 4
-          for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(&a.ml_part[part(p)]).x);
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int p = 0; p < parts; ++p) {
-            const float2 s = __ldcg(&a.ml_part[part(p)]);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.o_part + part(p) * D + d));
-            const float c = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
-            lsum += s.y * c;
-            acc.x += v.x * c;
-            acc.y += v.y * c;
-            acc.z += v.z * c;
-            acc.w += v.w * c;
-          }
-          const float inv = 1.f / lsum;
-          uint2 v = make_uint2(0u, 0u);
-          if (lsum > 0.f || lsum != lsum)
-            v = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-          *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) +
-                                    ((size_t)cc.b * a.nq + h0 + head) * D + d) = v;
-        }
-        if (threadIdx.x == 0) a.counters[c0] = 0;
+    if (!more_items) break;
+  }
+
+  // ---- cut items: the CTA that counts the last part joins them all. The
+  // first and the last item of a range can be cut.
+  const Cursor& tail = cc;
+  const bool cut0 = head.begin < r0 || head.end > r1;
+  const bool cut1 = tail.begin > head.begin && tail.end > r1;
+  if (cut0 || cut1) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const Cursor& c = threadIdx.x == 0 ? head : tail;
+      int last = 0;
+      if (threadIdx.x == 0 ? cut0 : cut1) {
+        int* counter = a.counters + first_cta(c.begin);
+        last = atomicAdd(counter, 1) == parts_of(c.begin, c.end) - 1;
+        if (last) *counter = 0;
       }
-      __syncthreads();  // last_part is written again at the next cut
+      joins_item[threadIdx.x] = last;
     }
-    if (cc.end >= r1) break;
+    __syncthreads();
+    __threadfence();
+    float2* mls = reinterpret_cast<float2*>(smem);  // the ring: every load has been consumed
+    for (int e = 0; e < 2; ++e) {
+      if (!joins_item[e]) continue;
+      const Cursor& c = e == 0 ? head : tail;
+      const int c0 = first_cta(c.begin), parts = parts_of(c.begin, c.end);
+      const int grp = c.sub % groups, h0 = (c.sub / groups) * G + grp * 8 * NT;
+      const int heads = min(8 * NT, G - grp * 8 * NT);
+      __syncthreads();
+      for (int i = threadIdx.x; i < parts * heads; i += kThreads)
+        mls[i] = __ldcg(a.ml_part + part_row(c0, i / heads) + i % heads);
+      __syncthreads();
+      for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
+        const int hd = i / (D / 4), d = i % (D / 4) * 4;
+        float M = -INFINITY, lsum = 0.f;
+        for (int p = 0; p < parts; ++p) M = fmaxf(M, mls[p * heads + hd].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) {
+          const float2 s = mls[p * heads + hd];
+          const float4 v = __ldcg(
+              reinterpret_cast<const float4*>(a.o_part + (part_row(c0, p) + hd) * D + d));
+          const float f = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
+          lsum += s.y * f;
+          acc.x += v.x * f;
+          acc.y += v.y * f;
+          acc.z += v.z * f;
+          acc.w += v.w * f;
+        }
+        store_out<T, D>(a, c.b, h0 + hd, d, acc, lsum);
+      }
+    }
   }
   if (!ok && lane == 0) {
     // loads that a failed wait left in flight must land before the CTA exits
