@@ -61,7 +61,7 @@ at::Tensor zeroed_counters(const at::Tensor& like, int64_t n) {
   static auto* pool = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
   std::lock_guard<std::mutex> lock(mu);
   at::Tensor& t = (*pool)[{like.device().index(), stream()}];
-  if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 1024)}, opt);
+  if (!t.defined() || t.numel() < n) t = at::zeros({std::max<int64_t>(n, 4096)}, opt);
   return t;
 }
 
@@ -170,17 +170,17 @@ at::Tensor paged_decode_attention(const at::Tensor& q_in, const at::Tensor& k_pa
   a.out = out.data_ptr();
   a.scale = scale_of(scale, a.D);
   a.status = status_ptr(status, q);
-  const int grid = num_sms();
+  const int sms = num_sms();
   TORCH_CHECK_VALUE((double)a.B * (a.max_pages * (a.page_size / 16.0) + 4) * a.nkv *
-                            ((a.nq / a.nkv + 15) / 16) < 2147483648.0 - 4096.0 * grid,
+                            ((a.nq / a.nkv + 15) / 16) < 2147483648.0 - 65536.0 * sms,
                     "the page table spans too many positions in all");
-  const int64_t parts = paged_decode_part_rows(a.nq, a.nkv, grid);
+  const int64_t parts = paged_decode_part_rows(a.nq, a.nkv, sms);
   const at::Tensor ws = at::empty({parts * (a.D + 2)}, q.options().dtype(at::kFloat));
-  const at::Tensor counters = zeroed_counters(q, grid);
+  const at::Tensor counters = zeroed_counters(q, paged_decode_counters(sms));
   a.o_part = ws.data_ptr<float>();
   a.ml_part = reinterpret_cast<float2*>(a.o_part + parts * a.D);
   a.counters = counters.data_ptr<int>();
-  check_rc(launch_paged_decode(a, grid, stream()), "paged_decode_attention");
+  check_rc(launch_paged_decode(a, sms, stream()), "paged_decode_attention");
   return out;
 }
 

@@ -40,20 +40,63 @@ namespace afd {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlk = 16;                 // keys of a block
 constexpr int kStages = 3;               // ring depth of a warp
-// Units of a range: blocks, and kItemCost more for an item (its queries, the
-// join of the warps: about what the HBM delivers of 4 blocks to an SM). A range
-// holds at least kMinRange of them, so that short sequences stay whole. A range
-// end near an item's end is moved there, within half a range where ranges are
-// short (up to kShortRange) and within kSnap units where they are long: a cut
-// costs a join through the workspace, an uneven range what it has more.
+constexpr int kCtasPerSm = 2;            // one joins and looks up while the other loads
+
+// Units of work: blocks, and kItemCost more for an item (its queries, the join
+// of the warps). With `even` the units per CTA, up to kEven of them each CTA
+// takes one range of that size, of at least kMinRange units (short sequences
+// stay whole). Above, the first range of a CTA has three quarters of its share
+// and the rest is left in ranges of half of what then remains, down to
+// smallest(), for whoever is done first: SMs get unequal shares of the HBM's rate
+// (equal static ranges ended between 104 and 150 us, median 127, where 950 MB
+// were read). The ranges' places follow from the lengths alone, and so do the
+// sums' order and the result's bits.
 constexpr int kItemCost = 4;
 constexpr int kMinRange = 20;
+constexpr int kEven = 96;
+constexpr int kZones = 8;                // sizes of ranges at most
+
+// A range end near an item's end is moved there, within half a range where
+// ranges are short (up to kShortRange) and within kSnap units where they are
+// long: a cut costs a join through the workspace, an uneven range what it has more.
 constexpr int kShortRange = 40;
 constexpr int kSnap = 8;
+constexpr int kPartBatch = 8;            // parts that a join has on their way at once
+
+// The ranges: zone z holds `grid` of them of size(z) units each.
+struct Ranges {
+  int even, grid;
+  __device__ __forceinline__ int first() const {
+    return even <= kEven ? max(kMinRange, even) : even / 4 * 3;
+  }
+  __device__ __forceinline__ int smallest() const { return max(kMinRange, even / 64); }
+  // Unit where range `id` starts.
+  __device__ __forceinline__ int start(int id) const {
+    int at = 0, size = first(), rest = even - size;
+    while (id >= grid) {
+      at += size * grid;
+      id -= grid;
+      size = max(smallest(), rest / 2);
+      rest -= size;
+    }
+    return at + id * size;
+  }
+  // Range that holds unit `at`.
+  __device__ __forceinline__ int id(int at) const {
+    int id = 0, size = first(), rest = even - size;
+    while (at >= size * grid) {
+      at -= size * grid;
+      id += grid;
+      size = max(smallest(), rest / 2);
+      rest -= size;
+    }
+    return id + at / size;
+  }
+};
 
 template <int D>
 struct Dec {
@@ -62,7 +105,7 @@ struct Dec {
   static constexpr int kStage = 2 * kTile;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kJoin = kWarps * 8 * D * 4;
-  static constexpr int kBytes = kRing + kJoin + 1024 /*align*/ + 1536 /*barriers, statistics*/;
+  static constexpr int kBytes = kRing + kJoin + 512 /*barriers, statistics*/;
 };
 
 // Float index of (warp, head, dim) in the join buffer: the heads of a quarter
@@ -102,10 +145,12 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    mma_16816_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -142,13 +187,11 @@ struct Place {  // of a range end: the item that it falls into, moved to an end 
 }  // namespace
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tk,
                         const __grid_constant__ CUtensorMap tv, PagedDecodeArgs a, int groups) {
   using C = Dec<D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // whole swizzle atoms
   float* join = reinterpret_cast<float*>(smem + C::kRing);           // [warps][8][D], join_at
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRing + C::kJoin);  // [warps][stages]
   float2* ml = reinterpret_cast<float2*>(full + kWarps * kStages);   // [warps][8]
@@ -157,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(place + 2);
   volatile int* joins_item = abort_flag + 1;                         // [2]
   volatile int* any_empty = joins_item + 2;
+  volatile int* next_range = any_empty + 1;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = a.nq / a.nkv, subs = a.nkv * groups;
@@ -172,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's range of the work: a scan over the sequences' extents
+  // ---- the extent of the work: a scan over the sequences
   auto extent = [](int len) { return len > 0 ? (len + kBlk - 1) / kBlk + kItemCost : 0; };
   const int chunk = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(a.B, (int)threadIdx.x * chunk), b1 = min(a.B, b0 + chunk);
@@ -198,37 +242,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += scan[w];
   }
   before += upto - mine;
-  const int range = max(kMinRange, (int)((total + gridDim.x - 1) / gridDim.x));
+  const Ranges ranges{(int)((total + gridDim.x - 1) / gridDim.x), (int)gridDim.x};
+  const int n_ranges = total > 0 ? ranges.id(total - 1) + 1 : 0;
   // a range end this near to an item's is moved there
-  const int snap = range <= kShortRange ? range / 2 : kSnap;
-  const bool works = (long long)blockIdx.x * range < total;
-  const int raw0 = works ? blockIdx.x * range : total;
-  if (works) {
-    for (int e = 0; e < 2; ++e) {
-      const int r = raw0 + e * range;
-      if (r < before || r - before >= mine) continue;
-      int at = before;
-      for (int b = b0; b < b1; ++b) {
-        const int len = checked_len(a.seq_lens[b], most, nullptr, 0);
-        const int ext = extent(len);
-        if (r - at < ext * subs) {
-          Place p;
-          p.b = b;
-          p.len = len;
-          p.sub = (r - at) / ext;
-          p.begin = at + p.sub * ext;
-          p.end = p.begin + ext;
-          p.at = r - p.begin <= snap ? p.begin : p.end - r <= snap ? p.end : r;
-          place[e] = p;
-          break;
-        }
-        at += ext * subs;
+  const int snap = ranges.first() <= kShortRange ? ranges.first() / 2 : kSnap;
+  // An item is cut at the range starts inside it that are not near its ends.
+  auto first_range = [&](int begin) { return ranges.id(begin + snap); };
+  auto parts_of = [&](int begin, int end) {
+    return ranges.id(end - snap - 1) - first_range(begin) + 1;
+  };
+  auto part_row = [&](int first, int p) {
+    return (size_t)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * 8 * NT;
+  };
+
+  uint8_t* ring = smem + warp * kStages * C::kStage;
+  uint64_t* bar = full + warp * kStages;
+  const float scale_log2 = a.scale * 1.4426950408889634f;
+  int issued = 0, used = 0;
+  bool ok = true;
+  for (int id = blockIdx.x; id < n_ranges; id = *next_range) {
+  // the CTA's next range, fetched when this one's loads are all on their way;
+  // the counter is zero again after the last fetch of the launch
+  unsigned fetched = 0;
+  auto fetch = [&]() {
+    if (threadIdx.x == 0 && n_ranges > (int)gridDim.x)
+      fetched =
+          atomicInc(reinterpret_cast<unsigned*>(a.counters + n_ranges), (unsigned)n_ranges - 1);
+  };
+  const int raw1 = id + 1 < n_ranges ? ranges.start(id + 1) : total;
+  for (int e = 0; e < 2; ++e) {
+    const int r = e == 0 ? ranges.start(id) : raw1;
+    if (r < before || r - before >= mine) continue;
+    int at = before;
+    for (int b = b0; b < b1; ++b) {
+      const int len = checked_len(a.seq_lens[b], most, nullptr, 0);
+      const int ext = extent(len);
+      if (r - at < ext * subs) {
+        Place p;
+        p.b = b;
+        p.len = len;
+        p.sub = (r - at) / ext;
+        p.begin = at + p.sub * ext;
+        p.end = p.begin + ext;
+        p.at = r - p.begin <= snap ? p.begin : p.end - r <= snap ? p.end : r;
+        place[e] = p;
+        break;
       }
+      at += ext * subs;
     }
   }
-  if (threadIdx.x == 0 && total - raw0 <= range) place[1].at = total;
+  if (threadIdx.x == 0 && raw1 == total) place[1].at = total;
   __syncthreads();
-  const int r0 = works ? place[0].at : total, r1 = place[1].at;
+  const int r0 = place[0].at, r1 = place[1].at;
 
   // the item after `c` and this CTA's portion of it
   auto take = [&](Cursor& c) {
@@ -269,10 +334,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Cursor cc = ic;
 
   // ---- the warp's loads, kStages blocks ahead
-  uint8_t* ring = smem + warp * kStages * C::kStage;
-  uint64_t* bar = full + warp * kStages;
   auto first_block = [&](const Cursor& c) { return c.j0 + ((warp - c.before) & (kWarps - 1)); };
-  int issued = 0, ij = 0, held = 0, page = 0, row = 0;
+  int ij = 0, held = 0, page = 0, row = 0;
   bool more = r0 < r1;
   // each lane holds the page of one of the next 32 blocks
   auto look_up = [&]() {
@@ -320,15 +383,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   find();
   for (int s = 0; s < kStages; ++s) issue();
 
-  // sequences without a key: zeros
-  if (*any_empty)
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-      if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
-        for (int i = threadIdx.x; i < a.nq * D / 8; i += kThreads)
-          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (size_t)b * a.nq * D)[i] =
-              make_uint4(0, 0, 0, 0);
-  if (r0 >= r1) return;
-
   // Q^T as the B operand: head lane / 4, dims 2 (lane % 4) + {0, 1, 8, 9} of 16
   uint32_t qf[NT][D / 16][2];
   auto load_q = [&](const Cursor& c) {
@@ -346,20 +400,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    q + (n * 8 + lane / 4) * D + kk * 16 + (lane % 4) * 2 + e * 8)
                              : 0u;
   };
-  load_q(cc);
-
-  // The cuts of an item lie at the multiples of `range` inside it that are not
-  // near its ends: CTA `first` has its first part, CTA first + p its part p.
-  auto first_cta = [&](int begin) { return (begin + snap) / range; };
-  auto parts_of = [&](int begin, int end) { return (end - snap - 1) / range - first_cta(begin) + 1; };
-  auto part_row = [&](int c0, int p) { return (size_t)(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * 8 * NT; };
+  if (r0 < r1) load_q(cc);
 
   // ---- the items of the range
-  const float scale_log2 = a.scale * 1.4426950408889634f;
+  if (r0 >= r1) fetch();
   const Cursor head = cc;
-  int used = 0;
-  bool ok = true;
-  for (;;) {
+  while (r0 < r1) {
     const int grp = cc.sub % groups, h0 = (cc.sub / groups) * G + grp * 8 * NT;
     const int heads = min(8 * NT, G - grp * 8 * NT);
     // lane: heads 2 (lane % 4) + {0, 1} of each tile
@@ -380,9 +426,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
       const uint32_t ks = smem_u32(ring + st * C::kStage), vs = ks + C::kTile;
       const int key0 = j * kBlk;
-      float s[NT][4];
+      // two chains of products, the even and the odd 16 dims
+      float s[NT][4], s2[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
       {
         const int r = (lane / 8 % 2) * 8 + lane % 8;
 #pragma unroll
@@ -391,9 +440,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ch = (kk % 4) * 2 + lane / 16;
           ldsm4(ks + (kk / 4) * C::kBox + r * 128 + ((ch ^ (r & 7)) << 4), kf);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<T>(s[n], kf, qf[n][kk][0], qf[n][kk][1]);
+          for (int n = 0; n < NT; ++n)
+            mma16816<T>(kk % 2 ? s2[n] : s[n], kf, qf[n][kk][0], qf[n][kk][1]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
       if (key0 + kBlk > cc.len) {
         // keys past the end: no weight, and finite values for it to meet
 #pragma unroll
@@ -472,9 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (more_items) {
       next_item(cc);
       load_q(cc);
+    } else {
+      fetch();
     }
     const bool cut = item.begin < r0 || item.end > r1;
-    const size_t row0 = (size_t)(item.begin < r0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1) * 8 * NT;
+    const size_t row0 = (size_t)(item.begin < r0 ? 2 * id : 2 * id + 1) * 8 * NT;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       __syncthreads();  // the buffer's last readers are done
@@ -520,11 +576,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!more_items) break;
   }
 
-  // ---- cut items: the CTA that counts the last part joins them all. The
+  // ---- cut items: whoever counts the last part joins them all. The
   // first and the last item of a range can be cut.
   const Cursor& tail = cc;
-  const bool cut0 = head.begin < r0 || head.end > r1;
-  const bool cut1 = tail.begin > head.begin && tail.end > r1;
+  const bool cut0 = r0 < r1 && (head.begin < r0 || head.end > r1);
+  const bool cut1 = r0 < r1 && tail.begin > head.begin && tail.end > r1;
   if (cut0 || cut1) {
     __threadfence();
     __syncthreads();
@@ -532,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Cursor& c = threadIdx.x == 0 ? head : tail;
       int last = 0;
       if (threadIdx.x == 0 ? cut0 : cut1) {
-        int* counter = a.counters + first_cta(c.begin);
+        int* counter = a.counters + first_range(c.begin);
         last = atomicAdd(counter, 1) == parts_of(c.begin, c.end) - 1;
         if (last) *counter = 0;
       }
@@ -540,38 +596,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     __threadfence();
-    float2* mls = reinterpret_cast<float2*>(smem);  // the ring: every load has been consumed
     for (int e = 0; e < 2; ++e) {
       if (!joins_item[e]) continue;
       const Cursor& c = e == 0 ? head : tail;
-      const int c0 = first_cta(c.begin), parts = parts_of(c.begin, c.end);
+      const int c0 = first_range(c.begin), parts = parts_of(c.begin, c.end);
       const int grp = c.sub % groups, h0 = (c.sub / groups) * G + grp * 8 * NT;
       const int heads = min(8 * NT, G - grp * 8 * NT);
-      __syncthreads();
-      for (int i = threadIdx.x; i < parts * heads; i += kThreads)
-        mls[i] = __ldcg(a.ml_part + part_row(c0, i / heads) + i % heads);
-      __syncthreads();
       for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
         const int hd = i / (D / 4), d = i % (D / 4) * 4;
         float M = -INFINITY, lsum = 0.f;
-        for (int p = 0; p < parts; ++p) M = fmaxf(M, mls[p * heads + hd].x);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int p = 0; p < parts; ++p) {
-          const float2 s = mls[p * heads + hd];
-          const float4 v = __ldcg(
-              reinterpret_cast<const float4*>(a.o_part + (part_row(c0, p) + hd) * D + d));
-          const float f = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
-          lsum += s.y * f;
-          acc.x += v.x * f;
-          acc.y += v.y * f;
-          acc.z += v.z * f;
-          acc.w += v.w * f;
+        for (int p0 = 0; p0 < parts; p0 += kPartBatch) {
+          float2 s[kPartBatch];
+          float4 v[kPartBatch];
+#pragma unroll
+          for (int p = 0; p < kPartBatch; ++p) {
+            const size_t at = part_row(c0, min(p0 + p, parts - 1)) + hd;
+            s[p] = __ldcg(a.ml_part + at);
+            v[p] = __ldcg(reinterpret_cast<const float4*>(a.o_part + at * D + d));
+            if (p0 + p >= parts) s[p].x = -INFINITY;
+          }
+          float m_new = M;
+#pragma unroll
+          for (int p = 0; p < kPartBatch; ++p) m_new = fmaxf(m_new, s[p].x);
+          const float f0 = M == -INFINITY ? 0.f : exp2_approx(M - m_new);
+          M = m_new;
+          lsum *= f0;
+          acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+          for (int p = 0; p < kPartBatch; ++p) {
+            const float f = s[p].x == -INFINITY ? 0.f : exp2_approx(s[p].x - M);
+            lsum += s[p].y * f;
+            acc.x += v[p].x * f;
+            acc.y += v[p].y * f;
+            acc.z += v[p].z * f;
+            acc.w += v[p].w * f;
+          }
         }
         store_out<T, D>(a, c.b, h0 + hd, d, acc, lsum);
       }
     }
   }
+  if (threadIdx.x == 0) *next_range = (int)(gridDim.x + fetched);
+  __syncthreads();
+  }  // ranges
+
+  // sequences without a key: zeros
+  __syncthreads();
+  if (*any_empty)
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
+        for (int i = threadIdx.x; i < a.nq * D / 8; i += kThreads)
+          reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + (size_t)b * a.nq * D)[i] =
+              make_uint4(0, 0, 0, 0);
   if (!ok && lane == 0) {
     // loads that a failed wait left in flight must land before the CTA exits
     volatile int no_abort = 0;
@@ -587,17 +664,27 @@ static int launch_one(const PagedDecodeArgs& a, int grid, int groups, const CUte
                       const CUtensorMap& tv, cudaStream_t s) {
   const auto kern = paged_decode_kernel<T, D, NT>;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), Dec<D>::kBytes);
+  if (e == cudaSuccess)  // room for both CTAs of an SM
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess)
     e = launch_k(kern, dim3(grid), dim3(kThreads), Dec<D>::kBytes, s, tk, tv, a, groups);
   return e == cudaSuccess ? 0 : 4000 + (int)e;
 }
 
-long long paged_decode_part_rows(int nq, int nkv, int grid) {
-  return 2ll * grid * (nq / nkv > 8 ? 16 : 8);
+// The most ranges that a launch makes (3/4, 1/8, 1/16, 1/32 and 1/64 of a
+// share, and one more 1/64 or two with the roundings).
+static int max_ranges(int num_sms) { return num_sms * kCtasPerSm * kZones; }
+
+long long paged_decode_part_rows(int nq, int nkv, int num_sms) {
+  return 2ll * max_ranges(num_sms) * (nq / nkv > 8 ? 16 : 8);
 }
 
-int launch_paged_decode(const PagedDecodeArgs& a, int grid, cudaStream_t s) {
+int paged_decode_counters(int num_sms) { return max_ranges(num_sms) + 1; }
+
+int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s) {
   if (a.B == 0) return 0;
+  const int grid = num_sms * kCtasPerSm;
   CUtensorMap tk, tv;
   // pool [pages, nkv * page_size, D]: a box is the 16 rows of a block
   const uint64_t dims[3] = {(uint64_t)a.D, (uint64_t)a.nkv * a.page_size, (uint64_t)a.num_pages};

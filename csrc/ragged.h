@@ -39,11 +39,12 @@ struct PagedDecodeArgs {
   int* status;              // optional [2]
   float* o_part;            // [paged_decode_part_rows, D]
   float2* ml_part;          // [paged_decode_part_rows]
-  int* counters;            // [grid], zero; left zero
+  int* counters;            // [paged_decode_counters], zero; left zero
 };
-// Rows of the workspace of a launch with `grid` CTAs.
-long long paged_decode_part_rows(int nq, int nkv, int grid);
-int launch_paged_decode(const PagedDecodeArgs& a, int grid, cudaStream_t s);
+// Workspace of a launch.
+long long paged_decode_part_rows(int nq, int nkv, int num_sms);
+int paged_decode_counters(int num_sms);
+int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s);
 
 // Causal attention of packed queries. Sequence i owns query rows
 // cu_q[i] .. cu_q[i+1] - 1; they are its last positions. Keys and values come
