@@ -174,11 +174,10 @@ at::Tensor paged_decode_attention(const at::Tensor& q_in, const at::Tensor& k_pa
   TORCH_CHECK_VALUE((double)a.B * (a.max_pages * (a.page_size / 16.0) + 4) * a.nkv *
                             ((a.nq / a.nkv + 15) / 16) < 2147483648.0 - 65536.0 * sms,
                     "the page table spans too many positions in all");
-  const int64_t parts = paged_decode_part_rows(a.nq, a.nkv, sms);
-  const at::Tensor ws = at::empty({parts * (a.D + 2)}, q.options().dtype(at::kFloat));
+  const at::Tensor parts = at::empty({(int64_t)paged_decode_part_bytes(a.nq, a.nkv, a.D, sms)},
+                                     q.options().dtype(at::kByte));
   const at::Tensor counters = zeroed_counters(q, paged_decode_counters(sms));
-  a.o_part = ws.data_ptr<float>();
-  a.ml_part = reinterpret_cast<float2*>(a.o_part + parts * a.D);
+  a.parts = parts.data_ptr();
   a.counters = counters.data_ptr<int>();
   check_rc(launch_paged_decode(a, sms, stream()), "paged_decode_attention");
   return out;

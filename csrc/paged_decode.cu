@@ -65,7 +65,6 @@ constexpr int kZones = 8;                // sizes of ranges at most
 // long: a cut costs a join through the workspace, an uneven range what it has more.
 constexpr int kShortRange = 40;
 constexpr int kSnap = 8;
-constexpr int kPartBatch = 8;            // parts that a join has on their way at once
 
 // The ranges: zone z holds `grid` of them of size(z) units each.
 struct Ranges {
@@ -104,8 +103,17 @@ struct Dec {
   static constexpr int kTile = kBlk * D * 2;          // K or V of a block
   static constexpr int kStage = 2 * kTile;
   static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kTasks = 8 * D / 4 / kThreads;  // float4 of 8 heads a thread joins
   static constexpr int kJoin = kWarps * 8 * D * 4;
   static constexpr int kBytes = kRing + kJoin + 512 /*barriers, statistics*/;
+};
+
+// A part in the workspace: (maximum, sum) of its heads, then their O.
+template <int D, int NT>
+struct Part {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kStats = kHeads * 8;
+  static constexpr int kBytes = kStats + kHeads * D * 4;
 };
 
 // Float index of (warp, head, dim) in the join buffer: the heads of a quarter
@@ -157,6 +165,16 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
   }
 }
 
+// Bulk copy of `bytes` (a multiple of 16, both ends 16-byte aligned).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Four output values of a head, from their weighted sum and the weights' sum.
 template <typename T, int D>
 __device__ __forceinline__ void store_out(const PagedDecodeArgs& a, int b, int h, int d, float4 acc,
@@ -197,7 +215,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   float2* ml = reinterpret_cast<float2*>(full + kWarps * kStages);   // [warps][8]
   int* scan = reinterpret_cast<int*>(ml + kWarps * 8);               // [warps]
   Place* place = reinterpret_cast<Place*>(scan + kWarps);            // [2]: of r0, r1
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(place + 2);
+  uint64_t* part_bar = reinterpret_cast<uint64_t*>(place + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(part_bar + 1);
   volatile int* joins_item = abort_flag + 1;                         // [2]
   volatile int* any_empty = joins_item + 2;
   volatile int* next_range = any_empty + 1;
@@ -207,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const int most = a.max_pages * a.page_size;
   if (threadIdx.x < kWarps * kStages) mbar_init(&full[threadIdx.x], 1);
   if (threadIdx.x == 0) {
+    mbar_init(part_bar, 1);
     *abort_flag = 0;
     *any_empty = 0;
     tma_prefetch_desc(&tk);
@@ -251,9 +271,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   auto parts_of = [&](int begin, int end) {
     return ranges.id(end - snap - 1) - first_range(begin) + 1;
   };
-  auto part_row = [&](int first, int p) {
-    return (size_t)(p == 0 ? 2 * first + 1 : 2 * (first + p)) * 8 * NT;
-  };
+  using P = Part<D, NT>;
+  auto part_at = [&](int slot) { return reinterpret_cast<uint8_t*>(a.parts) + (size_t)slot * P::kBytes; };
+  int part_phase = 0;
 
   uint8_t* ring = smem + warp * kStages * C::kStage;
   uint64_t* bar = full + warp * kStages;
@@ -530,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       fetch();
     }
     const bool cut = item.begin < r0 || item.end > r1;
-    const size_t row0 = (size_t)(item.begin < r0 ? 2 * id : 2 * id + 1) * 8 * NT;
+    uint8_t* part = part_at(item.begin < r0 ? 2 * id : 2 * id + 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       __syncthreads();  // the buffer's last readers are done
@@ -566,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           acc.w += v.w * c;
         }
         if (cut) {
-          *reinterpret_cast<float4*>(a.o_part + (row0 + hd) * D + d) = acc;
-          if (d == 0) a.ml_part[row0 + hd] = make_float2(M, lsum);
+          *reinterpret_cast<float4*>(part + P::kStats + (hd * D + d) * 4) = acc;
+          if (d == 0) reinterpret_cast<float2*>(part)[hd] = make_float2(M, lsum);
         } else {
           store_out<T, D>(a, item.b, h0 + hd, d, acc, lsum);
         }
@@ -582,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const bool cut0 = r0 < r1 && (head.begin < r0 || head.end > r1);
   const bool cut1 = r0 < r1 && tail.begin > head.begin && tail.end > r1;
   if (cut0 || cut1) {
+    fence_proxy_async_global();  // bulk copies read the parts
     __threadfence();
     __syncthreads();
     if (threadIdx.x < 2) {
@@ -602,38 +623,60 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const int c0 = first_range(c.begin), parts = parts_of(c.begin, c.end);
       const int grp = c.sub % groups, h0 = (c.sub / groups) * G + grp * 8 * NT;
       const int heads = min(8 * NT, G - grp * 8 * NT);
-      for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
-        const int hd = i / (D / 4), d = i % (D / 4) * 4;
-        float M = -INFINITY, lsum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < parts; p0 += kPartBatch) {
-          float2 s[kPartBatch];
-          float4 v[kPartBatch];
+      // the parts into the ring (every load of it has been consumed), as many
+      // at once as it holds
+      constexpr int kBatch = C::kRing / P::kBytes;
+      const uint32_t bytes = P::kStats + heads * D * 4;
+      float M[NT * C::kTasks], lsum[NT * C::kTasks];
+      float4 acc[NT * C::kTasks];
 #pragma unroll
-          for (int p = 0; p < kPartBatch; ++p) {
-            const size_t at = part_row(c0, min(p0 + p, parts - 1)) + hd;
-            s[p] = __ldcg(a.ml_part + at);
-            v[p] = __ldcg(reinterpret_cast<const float4*>(a.o_part + at * D + d));
-            if (p0 + p >= parts) s[p].x = -INFINITY;
-          }
-          float m_new = M;
-#pragma unroll
-          for (int p = 0; p < kPartBatch; ++p) m_new = fmaxf(m_new, s[p].x);
-          const float f0 = M == -INFINITY ? 0.f : exp2_approx(M - m_new);
-          M = m_new;
-          lsum *= f0;
-          acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
-#pragma unroll
-          for (int p = 0; p < kPartBatch; ++p) {
-            const float f = s[p].x == -INFINITY ? 0.f : exp2_approx(s[p].x - M);
-            lsum += s[p].y * f;
-            acc.x += v[p].x * f;
-            acc.y += v[p].y * f;
-            acc.z += v[p].z * f;
-            acc.w += v[p].w * f;
+      for (int t = 0; t < NT * C::kTasks; ++t) {
+        M[t] = -INFINITY;
+        lsum[t] = 0.f;
+        acc[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int p0 = 0; p0 < parts; p0 += kBatch) {
+        const int n = min(kBatch, parts - p0);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          fence_proxy_async_global();
+          mbar_arrive_expect_tx(part_bar, n * bytes);
+          for (int p = 0; p < n; ++p) {
+            const int k = p0 + p;
+            bulk_load(smem + p * P::kBytes, part_at(k == 0 ? 2 * c0 + 1 : 2 * (c0 + k)), bytes,
+                      part_bar);
           }
         }
-        store_out<T, D>(a, c.b, h0 + hd, d, acc, lsum);
+        if (!mbar_wait(part_bar, part_phase, abort_flag, a.status, 225)) ok = false;
+        part_phase ^= 1;
+#pragma unroll
+        for (int t = 0; t < NT * C::kTasks; ++t) {
+          const int i = t * kThreads + threadIdx.x, hd = i / (D / 4), d = i % (D / 4) * 4;
+          if (hd >= heads) break;
+          float m_new = M[t];
+          for (int p = 0; p < n; ++p)
+            m_new = fmaxf(m_new, reinterpret_cast<const float2*>(smem + p * P::kBytes)[hd].x);
+          const float f0 = M[t] == -INFINITY ? 0.f : exp2_approx(M[t] - m_new);
+          M[t] = m_new;
+          lsum[t] *= f0;
+          acc[t] = make_float4(acc[t].x * f0, acc[t].y * f0, acc[t].z * f0, acc[t].w * f0);
+          for (int p = 0; p < n; ++p) {
+            const uint8_t* at = smem + p * P::kBytes;
+            const float2 s = reinterpret_cast<const float2*>(at)[hd];
+            const float4 v = *reinterpret_cast<const float4*>(at + P::kStats + (hd * D + d) * 4);
+            const float f = s.x == -INFINITY ? 0.f : exp2_approx(s.x - m_new);
+            lsum[t] += s.y * f;
+            acc[t].x += v.x * f;
+            acc[t].y += v.y * f;
+            acc[t].z += v.z * f;
+            acc[t].w += v.w * f;
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT * C::kTasks; ++t) {
+        const int i = t * kThreads + threadIdx.x, hd = i / (D / 4), d = i % (D / 4) * 4;
+        if (hd < heads) store_out<T, D>(a, c.b, h0 + hd, d, acc[t], lsum[t]);
       }
     }
   }
@@ -654,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     volatile int no_abort = 0;
     for (int j = max(0, issued - kStages); j < issued; ++j)
       mbar_wait(&bar[j % kStages], (j / kStages) & 1, &no_abort, nullptr, 224, 100000000ull);
+    mbar_wait(part_bar, part_phase ^ 1, &no_abort, nullptr, 226, 100000000ull);
   }
 }
 
@@ -676,8 +720,8 @@ static int launch_one(const PagedDecodeArgs& a, int grid, int groups, const CUte
 // share, and one more 1/64 or two with the roundings).
 static int max_ranges(int num_sms) { return num_sms * kCtasPerSm * kZones; }
 
-long long paged_decode_part_rows(int nq, int nkv, int num_sms) {
-  return 2ll * max_ranges(num_sms) * (nq / nkv > 8 ? 16 : 8);
+long long paged_decode_part_bytes(int nq, int nkv, int D, int num_sms) {
+  return 2ll * max_ranges(num_sms) * (nq / nkv > 8 ? 16 : 8) * (8 + 4 * D);
 }
 
 int paged_decode_counters(int num_sms) { return max_ranges(num_sms) + 1; }

@@ -37,12 +37,11 @@ struct PagedDecodeArgs {
   float scale;              // > 0
   int elem;
   int* status;              // optional [2]
-  float* o_part;            // [paged_decode_part_rows, D]
-  float2* ml_part;          // [paged_decode_part_rows]
+  void* parts;              // [paged_decode_part_bytes], 16-byte aligned
   int* counters;            // [paged_decode_counters], zero; left zero
 };
 // Workspace of a launch.
-long long paged_decode_part_rows(int nq, int nkv, int num_sms);
+long long paged_decode_part_bytes(int nq, int nkv, int D, int num_sms);
 int paged_decode_counters(int num_sms);
 int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s);
 
