@@ -43,59 +43,21 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kBlk = 16;                 // keys of a block
-constexpr int kStages = 3;               // ring depth of a warp
+// Ring depth of a warp: 128 KB on their way to an SM. With three (192 KB) the
+// SMs' shares of the HBM's rate drift apart: 154 us against 150 for 950 MB.
+constexpr int kStages = 2;
 constexpr int kCtasPerSm = 2;            // one joins and looks up while the other loads
 
 // Units of work: blocks, and kItemCost more for an item (its queries, the join
-// of the warps). With `even` the units per CTA, up to kEven of them each CTA
-// takes one range of that size, of at least kMinRange units (short sequences
-// stay whole). Above, the first range of a CTA has three quarters of its share
-// and the rest is left in ranges of half of what then remains, down to
-// smallest(), for whoever is done first: SMs get unequal shares of the HBM's rate
-// (equal static ranges ended between 104 and 150 us, median 127, where 950 MB
-// were read). The ranges' places follow from the lengths alone, and so do the
-// sums' order and the result's bits.
+// of the warps). A range holds an equal share of them, at least kMinRange (short
+// sequences stay whole). A range end near an item's end is moved there, within
+// half a range where ranges are short (up to kShortRange) and within kSnap units
+// where they are long: a cut costs a join through the workspace, an uneven range
+// what it has more.
 constexpr int kItemCost = 4;
 constexpr int kMinRange = 20;
-constexpr int kEven = 96;
-constexpr int kZones = 8;                // sizes of ranges at most
-
-// A range end near an item's end is moved there, within half a range where
-// ranges are short (up to kShortRange) and within kSnap units where they are
-// long: a cut costs a join through the workspace, an uneven range what it has more.
 constexpr int kShortRange = 40;
 constexpr int kSnap = 8;
-
-// The ranges: zone z holds `grid` of them of size(z) units each.
-struct Ranges {
-  int even, grid;
-  __device__ __forceinline__ int first() const {
-    return even <= kEven ? max(kMinRange, even) : even / 4 * 3;
-  }
-  __device__ __forceinline__ int smallest() const { return max(kMinRange, even / 64); }
-  // Unit where range `id` starts.
-  __device__ __forceinline__ int start(int id) const {
-    int at = 0, size = first(), rest = even - size;
-    while (id >= grid) {
-      at += size * grid;
-      id -= grid;
-      size = max(smallest(), rest / 2);
-      rest -= size;
-    }
-    return at + id * size;
-  }
-  // Range that holds unit `at`.
-  __device__ __forceinline__ int id(int at) const {
-    int id = 0, size = first(), rest = even - size;
-    while (at >= size * grid) {
-      at -= size * grid;
-      id += grid;
-      size = max(smallest(), rest / 2);
-      rest -= size;
-    }
-    return id + at / size;
-  }
-};
 
 template <int D>
 struct Dec {
@@ -103,9 +65,9 @@ struct Dec {
   static constexpr int kTile = kBlk * D * 2;          // K or V of a block
   static constexpr int kStage = 2 * kTile;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kTasks = 8 * D / 4 / kThreads;  // float4 of 8 heads a thread joins
+  static constexpr int kTasks = (2 * D + kThreads - 1) / kThreads;  // float4 of 8 heads a thread joins
   static constexpr int kJoin = kWarps * 8 * D * 4;
-  static constexpr int kBytes = kRing + kJoin + 512 /*barriers, statistics*/;
+  static constexpr int kBytes = kRing + kJoin + kWarps * (8 * kStages + 64 + 4) + 128;
 };
 
 // A part in the workspace: (maximum, sum) of its heads, then their O.
@@ -219,7 +181,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(part_bar + 1);
   volatile int* joins_item = abort_flag + 1;                         // [2]
   volatile int* any_empty = joins_item + 2;
-  volatile int* next_range = any_empty + 1;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int G = a.nq / a.nkv, subs = a.nkv * groups;
@@ -255,43 +216,36 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
-  if (empty) *any_empty = 1;
+  if (empty) *any_empty = 1;  // read after the next barrier
   int total = 0, before = 0;
   for (int w = 0; w < kWarps; ++w) {
     if (w == warp) before = total;
     total += scan[w];
   }
   before += upto - mine;
-  const Ranges ranges{(int)((total + gridDim.x - 1) / gridDim.x), (int)gridDim.x};
-  const int n_ranges = total > 0 ? ranges.id(total - 1) + 1 : 0;
+  const int range = max(kMinRange, (int)((total + gridDim.x - 1) / gridDim.x));
   // a range end this near to an item's is moved there
-  const int snap = ranges.first() <= kShortRange ? ranges.first() / 2 : kSnap;
-  // An item is cut at the range starts inside it that are not near its ends.
-  auto first_range = [&](int begin) { return ranges.id(begin + snap); };
+  const int snap = range <= kShortRange ? range / 2 : kSnap;
+  // An item is cut at the multiples of `range` inside it that are not near its
+  // ends: CTA `first_cta` has its first part, the p-th after it part p.
+  auto first_cta = [&](int begin) { return (begin + snap) / range; };
   auto parts_of = [&](int begin, int end) {
-    return ranges.id(end - snap - 1) - first_range(begin) + 1;
+    return (end - snap - 1) / range - first_cta(begin) + 1;
   };
   using P = Part<D, NT>;
   auto part_at = [&](int slot) { return reinterpret_cast<uint8_t*>(a.parts) + (size_t)slot * P::kBytes; };
   int part_phase = 0;
+  const int id = blockIdx.x;
 
   uint8_t* ring = smem + warp * kStages * C::kStage;
   uint64_t* bar = full + warp * kStages;
   const float scale_log2 = a.scale * 1.4426950408889634f;
   int issued = 0, used = 0;
   bool ok = true;
-  for (int id = blockIdx.x; id < n_ranges; id = *next_range) {
-  // the CTA's next range, fetched when this one's loads are all on their way;
-  // the counter is zero again after the last fetch of the launch
-  unsigned fetched = 0;
-  auto fetch = [&]() {
-    if (threadIdx.x == 0 && n_ranges > (int)gridDim.x)
-      fetched =
-          atomicInc(reinterpret_cast<unsigned*>(a.counters + n_ranges), (unsigned)n_ranges - 1);
-  };
-  const int raw1 = id + 1 < n_ranges ? ranges.start(id + 1) : total;
+  const int raw0 = (int)min((long long)id * range, (long long)total);
+  const int raw1 = total - raw0 > range ? raw0 + range : total;
   for (int e = 0; e < 2; ++e) {
-    const int r = e == 0 ? ranges.start(id) : raw1;
+    const int r = e == 0 ? raw0 : raw1;
     if (r < before || r - before >= mine) continue;
     int at = before;
     for (int b = b0; b < b1; ++b) {
@@ -313,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   if (threadIdx.x == 0 && raw1 == total) place[1].at = total;
   __syncthreads();
-  const int r0 = place[0].at, r1 = place[1].at;
+  const int r0 = raw0 < total ? place[0].at : total, r1 = place[1].at;
 
   // the item after `c` and this CTA's portion of it
   auto take = [&](Cursor& c) {
@@ -423,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (r0 < r1) load_q(cc);
 
   // ---- the items of the range
-  if (r0 >= r1) fetch();
   const Cursor head = cc;
   while (r0 < r1) {
     const int grp = cc.sub % groups, h0 = (cc.sub / groups) * G + grp * 8 * NT;
@@ -546,8 +499,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if (more_items) {
       next_item(cc);
       load_q(cc);
-    } else {
-      fetch();
     }
     const bool cut = item.begin < r0 || item.end > r1;
     uint8_t* part = part_at(item.begin < r0 ? 2 * id : 2 * id + 1);
@@ -609,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const Cursor& c = threadIdx.x == 0 ? head : tail;
       int last = 0;
       if (threadIdx.x == 0 ? cut0 : cut1) {
-        int* counter = a.counters + first_range(c.begin);
+        int* counter = a.counters + first_cta(c.begin);
         last = atomicAdd(counter, 1) == parts_of(c.begin, c.end) - 1;
         if (last) *counter = 0;
       }
@@ -620,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     for (int e = 0; e < 2; ++e) {
       if (!joins_item[e]) continue;
       const Cursor& c = e == 0 ? head : tail;
-      const int c0 = first_range(c.begin), parts = parts_of(c.begin, c.end);
+      const int c0 = first_cta(c.begin), parts = parts_of(c.begin, c.end);
       const int grp = c.sub % groups, h0 = (c.sub / groups) * G + grp * 8 * NT;
       const int heads = min(8 * NT, G - grp * 8 * NT);
       // the parts into the ring (every load of it has been consumed), as many
@@ -680,12 +631,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
     }
   }
-  if (threadIdx.x == 0) *next_range = (int)(gridDim.x + fetched);
-  __syncthreads();
-  }  // ranges
 
   // sequences without a key: zeros
-  __syncthreads();
   if (*any_empty)
     for (int b = blockIdx.x; b < a.B; b += gridDim.x)
       if (checked_len(a.seq_lens[b], most, nullptr, 0) == 0)
@@ -716,15 +663,11 @@ static int launch_one(const PagedDecodeArgs& a, int grid, int groups, const CUte
   return e == cudaSuccess ? 0 : 4000 + (int)e;
 }
 
-// The most ranges that a launch makes (3/4, 1/8, 1/16, 1/32 and 1/64 of a
-// share, and one more 1/64 or two with the roundings).
-static int max_ranges(int num_sms) { return num_sms * kCtasPerSm * kZones; }
-
 long long paged_decode_part_bytes(int nq, int nkv, int D, int num_sms) {
-  return 2ll * max_ranges(num_sms) * (nq / nkv > 8 ? 16 : 8) * (8 + 4 * D);
+  return 2ll * num_sms * kCtasPerSm * (nq / nkv > 8 ? 16 : 8) * (8 + 4 * D);
 }
 
-int paged_decode_counters(int num_sms) { return max_ranges(num_sms) + 1; }
+int paged_decode_counters(int num_sms) { return num_sms * kCtasPerSm; }
 
 int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s) {
   if (a.B == 0) return 0;
