@@ -113,7 +113,7 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
     """Log-probabilities of the tokens `ids` (int64 [R]) under softmax(logits)
-    (bf16, fp16 or fp32 [R, V]), the entropy of each row, and its `top_k` (at
+    (bf16, fp16 or fp32 [R, V], V at most 2^21), the entropy of each row, and its `top_k` (at
     most 32) most likely tokens. Masked logits may be -inf. An id outside
     [0, V) gives NaN; a row without a finite maximum has no distribution and
     gives NaN throughout (its top_ids still follow the order of the logits, a

@@ -334,7 +334,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0
                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    _check(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be [rows, vocab]")
+    _check(logits.dim() == 2 and 1 <= logits.shape[1] <= 1 << 21,
+           "logits must be [rows, vocab] of 1 to 2097152 values a row")
     _check(logits.dtype in (torch.bfloat16, torch.float16, torch.float32),
            "logits must be bf16, fp16 or fp32")
     R, V = logits.shape

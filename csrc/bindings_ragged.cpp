@@ -331,8 +331,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
   TORCH_CHECK_VALUE(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat,
                     "logits must be bf16, fp16 or fp32");
   const int64_t R = logits_in.size(0), V = logits_in.size(1);
-  TORCH_CHECK_VALUE(V >= 1 && V < (1ll << 31) - 1024 && R < (1ll << 31),
-                    "logits must hold at least one value a row and fewer than 2^31");
+  TORCH_CHECK_VALUE(V >= 1 && V <= kMaxLogprobVocab && R < (1ll << 31),
+                    "logits must hold 1 to " + std::to_string(kMaxLogprobVocab) + " values a row");
   TORCH_CHECK_VALUE(ids.device() == logits_in.device() && ids.scalar_type() == at::kLong &&
                         ids.is_contiguous() && ids.numel() == R,
                     "ids must be a contiguous int64 tensor, one per row");
@@ -355,7 +355,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(
   a.R = (int)R;
   a.V = (int)V;
   a.top_k = (int)top_k;
-  check_rc(launch_token_logprobs(a, stream()), "token_logprobs");
+  const int splits = token_logprobs_splits(a.R, a.V, num_sms());
+  at::Tensor ws, counters;
+  if (splits > 1) {
+    ws = at::empty({(int64_t)token_logprobs_workspace(a.R, a.V, splits)},
+                   logits.options().dtype(at::kByte));
+    counters = zeroed_counters(logits, R);
+    a.counters = counters.data_ptr<int>();
+  }
+  check_rc(launch_token_logprobs(a, splits, splits > 1 ? ws.data_ptr() : nullptr, stream()),
+           "token_logprobs");
   return {logprob, entropy, top_ids, top_logprobs};
 }
 

@@ -117,10 +117,17 @@ struct TokenLogprobsArgs {
   float* entropy;           // [R]
   int64_t* top_ids;         // [R, top_k]
   float* top_logprobs;      // [R, top_k]
-  int R, V, top_k;          // top_k <= kMaxTopLogprobs
+  int R, V, top_k;          // V <= kMaxLogprobVocab, top_k <= kMaxTopLogprobs
   int elem;
+  int* counters;            // with splits > 1: [R], zero; left zero
+  float* parts;             // set by the launcher
+  uint32_t* block_keys;
 };
 constexpr int kMaxTopLogprobs = 32;
-int launch_token_logprobs(const TokenLogprobsArgs& a, cudaStream_t s);
+constexpr int kMaxLogprobVocab = 1 << 21;
+// CTAs per row, the bytes of workspace for them (16-byte aligned), the launch.
+int token_logprobs_splits(int R, int V, int num_sms);
+long long token_logprobs_workspace(int R, int V, int splits);
+int launch_token_logprobs(const TokenLogprobsArgs& a, int splits, void* ws, cudaStream_t s);
 
 }  // namespace afd
