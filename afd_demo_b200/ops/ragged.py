@@ -25,9 +25,16 @@ import torch
 from . import torch_ref
 
 
+_mod = None
+
+
 def _ext():
-    from . import ext
-    return ext()
+    """The extension, looked up once: these calls are short enough to notice."""
+    global _mod
+    if _mod is None:
+        from . import ext
+        _mod = ext()
+    return _mod
 
 
 class TokenLogprobs(NamedTuple):

@@ -8,6 +8,11 @@
 // store. The model's padded path rounds after the norm, the weight and each
 // RoPE product, as HF's eager code does; here a single rounding is both
 // closer to the formula and cheaper.
+//
+// Bound by the HBM: qkv is read and q, k, v are written once. D / 16 lanes take a
+// head, each with two runs of 8 elements (16 bytes) that RoPE pairs, and keep
+// the loads of kHeads heads of their token on the way at once; the table's
+// row and the page slot, of the token, come with them.
 
 #include "ragged.cuh"
 
@@ -15,76 +20,129 @@ namespace afd {
 
 namespace {
 
+constexpr int kHeads = 2;
+constexpr int kThreads = 128;
+
 template <typename T>
-__global__ void __launch_bounds__(256) norm_rope_kernel(NormRopeArgs a) {
+__device__ __forceinline__ void widen(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack2<T>(w[i]);
+    x[2 * i] = p.x;
+    x[2 * i + 1] = p.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
+  return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]),
+                    pack2<T>(x[6], x[7]));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(NormRopeArgs a, int groups) {
+  constexpr int kLanes = D / 16;  // of a head
   pdl_wait();
   pdl_trigger();
-  const int heads = a.nq + 2 * a.nkv;
-  const long long gw = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (gw >= (long long)a.T * heads) return;
-  const int t = (int)(gw / heads), h = (int)(gw % heads);
-  const int D = a.D, half = D / 2, per = half / 32;  // 1 or 2 pairs a lane
-  const T* src = reinterpret_cast<const T*>(a.qkv) + (size_t)t * a.qkv_row + (size_t)h * D;
-
-  T* dst = nullptr;
-  if (h < a.nq) {
-    dst = reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.nq + h) * D;
-  } else {
-    const bool is_k = h < a.nq + a.nkv;
-    const int kvh = is_k ? h - a.nq : h - a.nq - a.nkv;
-    if (a.k_pages != nullptr) {
-      const int64_t slot = a.slots[t];
-      if (slot < 0) return;
-      if (slot >= (int64_t)a.num_pages * a.page_size) {
-        if (lane == 0) report_status(a.status, kBoundsViolation, 201);
-        return;
-      }
-      T* pool = reinterpret_cast<T*>(is_k ? a.k_pages : a.v_pages);
-      dst = pool + (slot / a.page_size) * a.page_stride +
-            ((size_t)kvh * a.page_size + slot % a.page_size) * D;
-    } else {
-      if (!is_k) return;
-      dst = reinterpret_cast<T*>(a.k_out) + ((size_t)t * a.nkv + kvh) * D;
-    }
-    if (!is_k) {
-      for (int j = lane; j < D; j += 32) dst[j] = src[j];
-      return;
-    }
+  const long long unit = ((long long)blockIdx.x * kThreads + threadIdx.x) / kLanes;
+  const int sub = threadIdx.x % kLanes;
+  // a unit past the end repeats the last one without storing: its warp's
+  // shuffles stay whole
+  const bool live = unit < (long long)a.T * groups;
+  const int t = live ? (int)(unit / groups) : a.T - 1;
+  const int h0 = (int)(unit % groups) * kHeads;
+  const int heads = a.nq + (a.k_pages != nullptr ? 2 : 1) * a.nkv;
+  const T* src = reinterpret_cast<const T*>(a.qkv) + (size_t)t * a.qkv_row + sub * 8;
+  uint4 lo[kHeads], hi[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const T* x = src + (size_t)min(h0 + i, heads - 1) * D;
+    lo[i] = *reinterpret_cast<const uint4*>(x);
+    hi[i] = *reinterpret_cast<const uint4*>(x + D / 2);
   }
   int pos = a.positions[t];
+  T *kt = nullptr, *vt = nullptr;  // the token's k and v rows of kv head 0
+  int head_step = a.nkv;           // rows between kv heads
+  if (a.k_pages == nullptr) {
+    kt = reinterpret_cast<T*>(a.k_out) + (size_t)t * a.nkv * D;
+    head_step = 1;
+  } else {
+    const int64_t slot = a.slots[t];
+    if (slot >= (int64_t)a.num_pages * a.page_size) {
+      if (live && sub == 0) report_status(a.status, kBoundsViolation, 201);
+    } else if (slot >= 0) {
+      const int page = (int)(slot / a.page_size), row = (int)(slot - (int64_t)page * a.page_size);
+      const size_t at = (size_t)page * a.page_stride + (size_t)row * D;
+      kt = reinterpret_cast<T*>(a.k_pages) + at;
+      vt = reinterpret_cast<T*>(a.v_pages) + at;
+    }
+    head_step = a.page_size;
+  }
   if (pos < 0 || pos >= a.max_pos) {
-    if (lane == 0) report_status(a.status, kBoundsViolation, 202);
+    if (live && sub == 0) report_status(a.status, kBoundsViolation, 202);
     pos = min(max(pos, 0), a.max_pos - 1);
   }
-  const T* w = reinterpret_cast<const T*>(h < a.nq ? a.q_norm : a.k_norm);
-  float lo[2], hi[2], ss = 0.f;
-  for (int i = 0; i < per; ++i) {
-    lo[i] = to_f(src[lane + 32 * i]);
-    hi[i] = to_f(src[half + lane + 32 * i]);
-    ss += lo[i] * lo[i] + hi[i] * hi[i];
+  float c[8], s[8];
+  {
+    const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * D + sub * 8);
+    *reinterpret_cast<float4*>(c) = cs[0];
+    *reinterpret_cast<float4*>(c + 4) = cs[1];
+    *reinterpret_cast<float4*>(s) = cs[D / 8];
+    *reinterpret_cast<float4*>(s + 4) = cs[D / 8 + 1];
   }
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float r = rsqrtf(ss / (float)D + a.eps);
-  const float* cs = a.rope + (size_t)pos * D;
-  for (int i = 0; i < per; ++i) {
-    const int j = lane + 32 * i;
-    const float x = lo[i] * r * to_f(w[j]), y = hi[i] * r * to_f(w[half + j]);
-    dst[j] = from_f<T>(x * cs[j] - y * cs[half + j]);
-    dst[half + j] = from_f<T>(y * cs[j] + x * cs[half + j]);
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    const bool is_q = h < a.nq, is_v = h >= a.nq + a.nkv;
+    T* dst = is_q ? reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.nq + h) * D
+             : is_v ? (vt == nullptr ? nullptr : vt + (size_t)(h - a.nq - a.nkv) * head_step * D)
+                    : (kt == nullptr ? nullptr : kt + (size_t)(h - a.nq) * head_step * D);
+    float x[8], y[8], ss = 0.f;
+    widen<T>(lo[i], x);
+    widen<T>(hi[i], y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!live || h >= heads || dst == nullptr) continue;
+    uint4 vx = lo[i], vy = hi[i];
+    if (!is_v) {
+      const float r = rsqrtf(ss / (float)D + a.eps);
+      const T* w = reinterpret_cast<const T*>(is_q ? a.q_norm : a.k_norm) + sub * 8;
+      float wx[8], wy[8];
+      widen<T>(*reinterpret_cast<const uint4*>(w), wx);
+      widen<T>(*reinterpret_cast<const uint4*>(w + D / 2), wy);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float u = x[e] * r * wx[e], v = y[e] * r * wy[e];
+        x[e] = u * c[e] - v * s[e];
+        y[e] = v * c[e] + u * s[e];
+      }
+      vx = narrow<T>(x);
+      vy = narrow<T>(y);
+    }
+    *reinterpret_cast<uint4*>(dst + sub * 8) = vx;
+    *reinterpret_cast<uint4*>(dst + D / 2 + sub * 8) = vy;
   }
+}
+
+template <typename T>
+cudaError_t launch_one(const NormRopeArgs& a, cudaStream_t s) {
+  const int heads = a.nq + (a.k_pages != nullptr ? 2 : 1) * a.nkv;
+  const int groups = (heads + kHeads - 1) / kHeads;
+  const long long lanes = (long long)a.T * groups * (a.D / 16);
+  const dim3 grid((unsigned)((lanes + kThreads - 1) / kThreads));
+  return a.D == 128 ? launch_k(norm_rope_kernel<T, 128>, grid, dim3(kThreads), 0, s, a, groups)
+                    : launch_k(norm_rope_kernel<T, 64>, grid, dim3(kThreads), 0, s, a, groups);
 }
 
 }  // namespace
 
 int launch_norm_rope(const NormRopeArgs& a, cudaStream_t s) {
   if (a.T == 0) return 0;
-  const long long warps = (long long)a.T * (a.nq + 2 * a.nkv);
-  const unsigned grid = (unsigned)((warps + 7) / 8);
   const cudaError_t e =
-      a.elem == kElemBf16
-          ? launch_k(norm_rope_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, a)
-          : launch_k(norm_rope_kernel<__half>, dim3(grid), dim3(256), 0, s, a);
+      a.elem == kElemBf16 ? launch_one<__nv_bfloat16>(a, s) : launch_one<__half>(a, s);
   return e == cudaSuccess ? 0 : 4000 + (int)e;
 }
 

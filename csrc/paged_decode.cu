@@ -554,20 +554,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const bool cut1 = r0 < r1 && tail.begin > head.begin && tail.end > r1;
   if (cut0 || cut1) {
     fence_proxy_async_global();  // bulk copies read the parts
-    __threadfence();
     __syncthreads();
     if (threadIdx.x < 2) {
       const Cursor& c = threadIdx.x == 0 ? head : tail;
       int last = 0;
       if (threadIdx.x == 0 ? cut0 : cut1) {
         int* counter = a.counters + first_cta(c.begin);
-        last = atomicAdd(counter, 1) == parts_of(c.begin, c.end) - 1;
+        last = count_arrival(counter) == parts_of(c.begin, c.end) - 1;
         if (last) *counter = 0;
       }
       joins_item[threadIdx.x] = last;
     }
     __syncthreads();
-    __threadfence();
     for (int e = 0; e < 2; ++e) {
       if (!joins_item[e]) continue;
       const Cursor& c = e == 0 ? head : tail;

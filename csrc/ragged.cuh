@@ -81,6 +81,18 @@ inline int encode_map16(CUtensorMap* m, const void* base, int elem, int rank, co
   return r == CUDA_SUCCESS ? 0 : 100 + (int)r;
 }
 
+// Counts this CTA's arrival, by one thread after a barrier of the CTA: its
+// writes before the barrier are visible to the CTA that counts the last arrival,
+// after that CTA's next barrier.
+__device__ __forceinline__ int count_arrival(int* counter) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+               : "=r"(old)
+               : "l"(counter)
+               : "memory");
+  return old;
+}
+
 // A sequence length read from the device: values outside [0, most] are
 // recorded and count as zero.
 __device__ __forceinline__ int checked_len(int len, int most, int* status, int where) {

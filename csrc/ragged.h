@@ -121,7 +121,7 @@ struct TokenLogprobsArgs {
   int elem;
   int* counters;            // with splits > 1: [R], zero; left zero
   float* parts;             // set by the launcher
-  uint32_t* block_keys;
+  float* block_max;
 };
 constexpr int kMaxTopLogprobs = 32;
 constexpr int kMaxLogprobVocab = 1 << 21;

@@ -12,9 +12,10 @@
 // What bounds it is reading the logits once. A warp takes blocks of 512
 // elements, the next block on its way while one is summed: the block's maximum
 // by one warp reduction (a running maximum of the warp's, so that sums are
-// rescaled only when it moves), then an exponential and four adds and multiplies
-// per element, in pairs. x - m comes before the factor log2(e): a mask of the
-// type's lowest value would leave fp32's range with it.
+// rescaled only when it moves), then an exponential, two multiply-adds and an add
+// per element, in pairs. The loop issues about 100 instructions for a block's 16
+// exponentials a lane, so that the exponentials (a quarter of a warp's lanes a
+// cycle) and not the issue come next after the memory.
 //
 // The top tokens cost the pass nothing but the block maxima, which it has
 // anyway and leaves behind: the k blocks with the largest maxima (the earlier
@@ -39,7 +40,7 @@ constexpr int kBlock = 512;             // elements of a block: 16 a lane
 constexpr int kMaxBlocks = kMaxLogprobVocab / kBlock;
 constexpr int kList = 2048;             // elements above the threshold at most (see refine)
 constexpr int kTies = 256;              // elements at the threshold kept before k are picked in order
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Floats in an order that unsigned integers have, NaN last; never 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -82,23 +83,25 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
+// A warp's blocks on their way, in shared memory: each lane copies what it will
+// read, so no lane waits for another.
+constexpr int kStages = 4;
+template <typename T>
+struct Ring {
+  static constexpr int kParts = sizeof(T);  // 16-byte parts of a lane
+  uint4 part[kStages][kParts][32];
+};
 
-// A lane's 16 elements of a block: two runs of 8 neighbours, 256 elements apart,
-// where rows are 16-byte aligned (kVec); every 32nd element elsewhere.
+// A lane's 16 elements of a block: runs of 16 bytes, a warp's side by side, where
+// rows are 16-byte aligned (kVec); every 32nd element elsewhere.
 template <typename T, bool kVec>
 struct Lane {
   static constexpr int kWords = 16 * sizeof(T) / 4;
   uint32_t w[kWords];
 
   static __device__ __forceinline__ int index(int lane, int e) {
-    return kVec ? (e / 8) * 256 + lane * 8 + e % 8 : e * 32 + lane;
+    constexpr int n = 16 / (int)sizeof(T);  // of a run
+    return kVec ? (e / n) * (32 * n) + lane * n + e % n : e * 32 + lane;
   }
   __device__ __forceinline__ void set(int e, float v) {
     if constexpr (sizeof(T) == 4) {
@@ -113,16 +116,13 @@ struct Lane {
   __device__ __forceinline__ void load(const T* x, int at, int V, int lane) {
     if (kVec && at + kBlock <= V) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int q = 0; q < kWords / 8; ++q) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + at + h * 256 + lane * 8) + q);
-          const int o = h * (kWords / 2) + q * 4;
-          w[o] = v.x;
-          w[o + 1] = v.y;
-          w[o + 2] = v.z;
-          w[o + 3] = v.w;
-        }
+      for (int q = 0; q < kWords / 4; ++q) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + at) + q * 32 + lane);
+        w[q * 4] = v.x;
+        w[q * 4 + 1] = v.y;
+        w[q * 4 + 2] = v.z;
+        w[q * 4 + 3] = v.w;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -135,11 +135,59 @@ struct Lane {
       }
     }
   }
+  __device__ __forceinline__ void take(const Ring<T>& ring, int stage, int lane) {
+#pragma unroll
+    for (int q = 0; q < Ring<T>::kParts; ++q) {
+      const uint4 v = ring.part[stage][q][lane];
+      w[q * 4] = v.x;
+      w[q * 4 + 1] = v.y;
+      w[q * 4 + 2] = v.z;
+      w[q * 4 + 3] = v.w;
+    }
+  }
   __device__ __forceinline__ float2 pair(int p) const {
     if constexpr (sizeof(T) == 4)
       return make_float2(__uint_as_float(w[2 * p]), __uint_as_float(w[2 * p + 1]));
     else
       return unpack2<T>(w[p]);
+  }
+  // The largest element, NaN if there is one; 16-bit types two at a time.
+  __device__ __forceinline__ float most() const {
+    if constexpr (sizeof(T) == 4) {
+      auto v = [&](int i) { return __uint_as_float(w[i]); };
+      float x = max3n(v(0), v(1), v(2)), y = max3n(v(3), v(4), v(5));
+      x = max3n(max3n(x, v(6), v(7)), v(8), v(9));
+      y = max3n(max3n(y, v(10), v(11)), v(12), v(13));
+      return max3n(max3n(x, v(14), v(15)), y, y);
+    } else {
+      const uint32_t m = max2n(max2n(max2n(w[0], w[1]), max2n(w[2], w[3])),
+                               max2n(max2n(w[4], w[5]), max2n(w[6], w[7])));
+      const float2 v = unpack2<T>(m);
+      return max3n(v.x, v.y, v.y);
+    }
+  }
+  static __device__ __forceinline__ uint32_t max2n(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  // -inf as a number far below every maximum that Sums::add takes (kFar).
+  __device__ __forceinline__ void lift() {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        asm("max.bf16x2 %0, %0, %1;" : "+r"(w[p]) : "r"(0xf149f149u));  // -1e30
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        asm("max.f16x2 %0, %0, %1;" : "+r"(w[p]) : "r"(0xfbfffbffu));  // -65504
+    } else {
+#pragma unroll
+      for (int p = 0; p < 16; ++p) w[p] = __float_as_uint(fmaxf(__uint_as_float(w[p]), -1e30f));
+    }
   }
 };
 
@@ -160,45 +208,128 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   return {m, a.z * ca + b.z * cb, ca * (a.s + a.z * da) + cb * (b.s + b.z * db)};
 }
 
+// A lane's running sums, all lanes of a warp with the same m. S is kept over
+// log2(e), and so is the exponent's m: t = x log2(e) - m2.
+template <typename T>
+struct Running {
+  // Below (or, bf16 and fp32, above) these, two values of T that differ do so by
+  // 32 at least: the maximum's equals have the weight 1 and the others 1e-14 at most.
+  static constexpr float kFarLow = std::is_same<T, __half>::value ? -60000.f : -0.9e30f;
+  static constexpr float kFarHigh = 0.9e30f;
+  float m = -INFINITY, m2 = -INFINITY;
+  float2 z = {0.f, 0.f}, s = {0.f, 0.f};
+
+  // A block whose largest element over the warp is `most`.
+  template <typename Block>
+  __device__ __forceinline__ void add(Block& b, float most) {
+    if (!(most <= m)) {
+      if (most != most) most = INFINITY;
+      const float d = fmaxf(m - most, kGone) * kLog2e, c = exp2_approx(d);
+      s = make_float2((s.x + z.x * d) * c, (s.y + z.y * d) * c);
+      z = make_float2(z.x * c, z.y * c);
+      m = most;
+      m2 = m * kLog2e;
+    }
+    if (m > kFarLow && m < kFarHigh) {
+      b.lift();
+      const float2 l2 = make_float2(kLog2e, kLog2e), nm = make_float2(-m2, -m2);
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float2 t = fma2(b.pair(p), l2, nm);
+        const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+        z = add2(z, e);
+        s = fma2(e, t, s);
+      }
+    } else if (m > -INFINITY) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float2 v = b.pair(p);
+        z.x += v.x == m ? 1.f : 0.f;
+        z.y += v.y == m ? 1.f : 0.f;
+      }
+    }
+  }
+  // Over the warp. The exponents had the rounded m2 where m log2(e) is meant;
+  // both sums are put right for the difference.
+  __device__ __forceinline__ Sums all() const {
+    Sums r = {m, z.x + z.y, s.x + s.y};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
+      r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+    }
+    if (m > kFarLow && m < kFarHigh) {
+      const float off = fmaf(-m, kLog2e, m2), c = exp2f(off);
+      r.s = (r.s + r.z * off) * c;
+      r.z *= c;
+    }
+    r.s *= kLn2;
+    return r;
+  }
+};
+
+template <typename T>
 struct Shared {
   Sums sums[kWarps];
   int sel[kMaxTopLogprobs];
   uint32_t thr;
   int n_sel, n_list, n_ties, last;
-  uint32_t most[kThreads];
-  unsigned long long list[kList + kTies];
-  uint32_t keys[1];  // [blocks], of the dynamic part
+  union {
+    Ring<T> ring[kWarps];                             // while the row is read
+    struct {                                          // after it
+      unsigned long long list[kList + kTies];
+      uint32_t most[kThreads];
+    };
+  };
+  union {  // [blocks], of the dynamic part
+    float block_max[1];
+    uint32_t keys[1];
+  };
 };
 
 // The top_k elements of row x as (key, ~index) in sh.list, unsorted, from the
 // block maxima in sh.keys; returns how many were listed (top_k at least).
 template <typename T, bool kVec>
-__device__ int list_top(Shared& sh, const T* x, int V, int n_blocks, int top_k) {
+__device__ int list_top(Shared<T>& sh, const T* x, int V, int n_blocks, int top_k) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (warp == 0) {
-    // top_k rounds: the largest key left, the first block of equals
+    // top_k rounds: the largest key left, the first block of equals. The lanes
+    // hold the keys of up to 512 blocks in registers.
     const int n = min(top_k, n_blocks);
-    uint32_t best = 0;
-    int at = 0;
-    auto look = [&]() {
-      best = 0;
-      for (int i = lane; i < n_blocks; i += 32)
-        if (sh.keys[i] > best) {
-          best = sh.keys[i];
-          at = i;
-        }
-    };
-    look();
+    const bool held = n_blocks <= 32 * 16;
+    uint32_t key[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      key[i] = held && i * 32 + lane < n_blocks ? sh.keys[i * 32 + lane] : 0;
     uint32_t k = 0;
     for (int r = 0; r < n; ++r) {
-      k = __reduce_max_sync(0xffffffffu, best);
-      const int b = (int)__reduce_min_sync(0xffffffffu, best == k ? (unsigned)at : 0xffffffffu);
-      if (lane == 0) sh.sel[r] = b;
-      if (best == k && at == b) {
-        sh.keys[b] = 0;
-        look();
+      uint32_t best = 0;
+      if (held) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) best = max(best, key[i]);
+      } else {
+        for (int i = lane; i < n_blocks; i += 32) best = max(best, sh.keys[i]);
       }
-      __syncwarp();
+      k = __reduce_max_sync(0xffffffffu, best);
+      unsigned at = 0xffffffffu;
+      if (held) {
+#pragma unroll
+        for (int i = 15; i >= 0; --i)
+          if (key[i] == k) at = i * 32 + lane;
+      } else if (best == k) {
+        for (int i = n_blocks - 1; i >= 0; --i)
+          if (i % 32 == lane && sh.keys[i] == k) at = i;
+      }
+      const int b = (int)__reduce_min_sync(0xffffffffu, at);
+      if (lane == 0) sh.sel[r] = b;
+      if (held) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i * 32 + lane == b) key[i] = 0;
+      } else {
+        if (b % 32 == lane) sh.keys[b] = 0;
+        __syncwarp();
+      }
     }
     if (lane == 0) {
       sh.n_sel = n;
@@ -208,28 +339,42 @@ __device__ int list_top(Shared& sh, const T* x, int V, int n_blocks, int top_k) 
   }
   __syncthreads();
   const int n_sel = sh.n_sel;
-  // every element of the picked blocks, with its key (0 past the row's end)
+  // f(v, at) for the lane's elements of every picked block, kBatch blocks of the
+  // warp on their way at once
   auto each = [&](auto&& f) {
-    for (int b = warp; b < n_sel; b += kWarps) {
-      Lane<T, kVec> v;
-      const int at = sh.sel[b] * kBlock;
-      v.load(x, at, V, lane);
+    constexpr int kBatch = 2;
+    for (int b0 = warp; b0 < n_sel; b0 += kBatch * kWarps) {
+      Lane<T, kVec> v[kBatch];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float2 p = v.pair(e / 2);
-        const int i = at + Lane<T, kVec>::index(lane, e);
-        f(i < V ? order_of(e % 2 ? p.y : p.x) : 0u, i);
-      }
+      for (int j = 0; j < kBatch; ++j)
+        if (b0 + j * kWarps < n_sel) v[j].load(x, sh.sel[b0 + j * kWarps] * kBlock, V, lane);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (b0 + j * kWarps < n_sel) f(v[j], sh.sel[b0 + j * kWarps] * kBlock);
     }
   };
+  // the key of element e, 0 past the row's end
+  auto key_of = [&](const Lane<T, kVec>& v, int at, int e) {
+    const float2 p = v.pair(e / 2);
+    return at + Lane<T, kVec>::index(lane, e) < V ? order_of(e % 2 ? p.y : p.x) : 0u;
+  };
   auto collect = [&]() {
-    const uint32_t thr = sh.thr;
-    each([&](uint32_t k, int i) {
-      if (k >= thr && k != 0) {
+    const uint32_t thr = max(sh.thr, 1u);
+    each([&](const Lane<T, kVec>& v, int at) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t k = key_of(v, at, e);
+        if (k < thr) continue;
         const bool tie = k == thr;
-        const int at = atomicAdd(tie ? &sh.n_ties : &sh.n_list, 1);
-        if (at < (tie ? kTies : kList))
-          sh.list[tie ? kList + at : at] = ((unsigned long long)k << 32) | (uint32_t)~i;
+        int* counter = tie ? &sh.n_ties : &sh.n_list;
+        const int most = tie ? kTies : kList;
+        // past its end the list does not count on: a mask of -inf can leave
+        // thousands of ties
+        if (*(volatile int*)counter > most) continue;
+        const int i = atomicAdd(counter, 1);
+        if (i < most)
+          sh.list[tie ? kList + i : i] =
+              ((unsigned long long)k << 32) | (uint32_t)~(at + Lane<T, kVec>::index(lane, e));
       }
     });
     __syncthreads();
@@ -240,7 +385,10 @@ __device__ int list_top(Shared& sh, const T* x, int V, int n_blocks, int top_k) 
     // top_k - 1 <= 31 threads hold elements above it, of the 64 at most that a
     // thread sees: they fit the list.
     uint32_t mine = 0;
-    each([&](uint32_t k, int) { mine = max(mine, k); });
+    each([&](const Lane<T, kVec>& v, int at) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mine = max(mine, key_of(v, at, e));
+    });
     sh.most[threadIdx.x] = mine;
     __syncthreads();
     int rank = 0;
@@ -289,10 +437,10 @@ __device__ int list_top(Shared& sh, const T* x, int V, int n_blocks, int top_k) 
 }
 
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 5)
     token_logprobs_kernel(TokenLogprobsArgs a, int splits, int n_blocks) {
   extern __shared__ __align__(16) uint8_t raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  Shared<T>& sh = *reinterpret_cast<Shared<T>*>(raw);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int r = blockIdx.x / splits, split = blockIdx.x % splits;
   pdl_wait();
@@ -300,55 +448,56 @@ __global__ void __launch_bounds__(kThreads, 4)
   const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)r * a.row;
   const int first = (int)((long long)n_blocks * split / splits);
   const int end = (int)((long long)n_blocks * (split + 1) / splits);
-  uint32_t* keys = splits > 1 ? a.block_keys + (size_t)r * n_blocks : sh.keys;
+  float* keys = splits > 1 ? a.block_max + (size_t)r * n_blocks : sh.block_max;
 
-  float m = -INFINITY;  // of this warp's blocks
-  float2 z2 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);
-  Lane<T, kVec> cur, next;
+  Running<T> run;
+  // whole blocks of the warp through the ring, kStages - 1 ahead
+  Ring<T>& ring = sh.ring[warp];
+  const int whole = kVec ? min(end, a.V / kBlock) : 0;
   int b = first + warp;
-  if (b < end) cur.load(x, b * kBlock, a.V, lane);
-  for (; b < end; b += kWarps) {
-    if (b + kWarps < end) next.load(x, (b + kWarps) * kBlock, a.V, lane);
-    float2 v[8];
-#pragma unroll
-    for (int p = 0; p < 8; ++p) v[p] = cur.pair(p);
-    float mx = max3n(v[0].x, v[0].y, v[1].x);
-    float my = max3n(v[1].y, v[2].x, v[2].y);
-#pragma unroll
-    for (int p = 3; p < 7; p += 2) {
-      mx = max3n(mx, v[p].x, v[p].y);
-      my = max3n(my, v[p + 1].x, v[p + 1].y);
+  int ahead = b, stage = 0;
+  const T* src = x + (size_t)b * kBlock + lane * (16 / (int)sizeof(T));
+  auto fetch = [&](int st) {
+    if (ahead < whole) {
+      const uint32_t dst = smem_u32(&ring.part[st][0][lane]);
+      if constexpr (sizeof(T) == 2)
+        asm volatile(
+            "cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+            "cp.async.cg.shared.global [%0 + 512], [%1 + 512], 16;" ::"r"(dst), "l"(src)
+            : "memory");
+      else
+        asm volatile(
+            "cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+            "cp.async.cg.shared.global [%0 + 512], [%1 + 512], 16;\n\t"
+            "cp.async.cg.shared.global [%0 + 1024], [%1 + 1024], 16;\n\t"
+            "cp.async.cg.shared.global [%0 + 1536], [%1 + 1536], 16;" ::"r"(dst), "l"(src)
+            : "memory");
     }
-    mx = warp_max_nan(max3n(max3n(mx, v[7].x, v[7].y), my, my));
-    if (a.top_k > 0 && lane == 0) keys[b] = order_of(mx);
-    if (mx != mx) m = INFINITY;
-    if (mx > -INFINITY && m < INFINITY) {
-      if (mx > m) {
-        const float d = fmaxf(m - mx, kGone), c = exp_neg(d);
-        s2 = make_float2((s2.x + z2.x * d) * c, (s2.y + z2.y * d) * c);
-        z2 = make_float2(z2.x * c, z2.y * c);
-        m = mx;
-      }
-      const float2 nm = make_float2(-m, -m), l2 = make_float2(kLog2e, kLog2e);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ahead += kWarps;
+    src += kWarps * kBlock;
+  };
+  auto block = [&](Lane<T, kVec>& v) {
+    const float most = warp_max_nan(v.most());
+    if (a.top_k > 0 && lane == 0) keys[b] = most;
+    run.add(v, most);
+  };
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        float2 d = add2(v[p], nm);
-        d.x = fmaxf(d.x, kGone);
-        d.y = fmaxf(d.y, kGone);
-        const float2 t = mul2(d, l2);
-        const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-        z2 = add2(z2, e);
-        s2 = fma2(e, d, s2);
-      }
-    }
-    cur = next;
+  for (int st = 0; st < kStages - 1; ++st) fetch(st);
+  for (; b < whole; b += kWarps) {
+    fetch((stage + kStages - 1) % kStages);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    Lane<T, kVec> v;
+    v.take(ring, stage, lane);
+    stage = (stage + 1) % kStages;
+    block(v);
   }
-  Sums mine = {m, z2.x + z2.y, s2.x + s2.y};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {  // one m for the whole warp
-    mine.z += __shfl_xor_sync(0xffffffffu, mine.z, o);
-    mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
+  for (; b < end; b += kWarps) {  // the row's last block, or rows off the 16-byte grid
+    Lane<T, kVec> v;
+    v.load(x, b * kBlock, a.V, lane);
+    block(v);
   }
+  const Sums mine = run.all();
   if (lane == 0) sh.sums[warp] = mine;
   __syncthreads();
   Sums all = sh.sums[0];
@@ -358,20 +507,21 @@ __global__ void __launch_bounds__(kThreads, 4)
     float* part = a.parts + ((size_t)r * splits + split) * 4;
     if (threadIdx.x == 0)
       *reinterpret_cast<float4*>(part) = make_float4(all.m, all.z, all.s, 0.f);
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-      sh.last = atomicAdd(&a.counters[r], 1) == splits - 1;
+      sh.last = count_arrival(&a.counters[r]) == splits - 1;
       if (sh.last) a.counters[r] = 0;
     }
     __syncthreads();
     if (!sh.last) return;
-    __threadfence();
+    const float4* parts = reinterpret_cast<const float4*>(a.parts) + (size_t)r * splits;
+    float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (lane < splits) p = __ldcg(parts + lane);
     if (a.top_k > 0)
-      for (int i = threadIdx.x; i < n_blocks; i += kThreads) sh.keys[i] = __ldcg(keys + i);
-    all = {-INFINITY, 0.f, 0.f};
-    for (int i = lane; i < splits; i += 32) {
-      const float4 p = __ldcg(reinterpret_cast<const float4*>(a.parts) + (size_t)r * splits + i);
+      for (int i = threadIdx.x; i < n_blocks; i += kThreads) sh.block_max[i] = __ldcg(keys + i);
+    all = {p.x, p.y, p.z};
+    for (int i = lane + 32; i < splits; i += 32) {
+      p = __ldcg(parts + i);
       all = join(all, {p.x, p.y, p.z});
     }
 #pragma unroll
@@ -393,6 +543,8 @@ __global__ void __launch_bounds__(kThreads, 4)
     a.entropy[r] = none ? NAN : lz - all.s / all.z;
   }
   if (a.top_k == 0) return;
+  for (int i = threadIdx.x; i < n_blocks; i += kThreads) sh.keys[i] = order_of(sh.block_max[i]);
+  __syncthreads();
   const int n = list_top<T, kVec>(sh, x, a.V, n_blocks, a.top_k);
   for (int c = threadIdx.x; c < n; c += kThreads) {
     const unsigned long long k = sh.list[c];
@@ -407,12 +559,12 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 template <typename T>
 int launch_one(const TokenLogprobsArgs& a, int splits, int n_blocks, cudaStream_t s) {
-  const size_t bytes = sizeof(Shared) + (size_t)(a.top_k > 0 ? n_blocks : 0) * 4;
+  const size_t bytes = sizeof(Shared<T>) + (size_t)(a.top_k > 0 ? n_blocks : 0) * 4;
   const bool vec = ((uintptr_t)a.logits & 15) == 0 &&
                    (a.R == 1 || a.row * (long long)sizeof(T) % 16 == 0);
   const auto kern = vec ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern),
-                                       (int)(sizeof(Shared) + kMaxBlocks * 4));
+                                       (int)(sizeof(Shared<T>) + kMaxBlocks * 4));
   if (e == cudaSuccess)
     e = launch_k(kern, dim3((unsigned)(a.R * splits)), dim3(kThreads), bytes, s, a, splits,
                  n_blocks);
@@ -423,10 +575,10 @@ int blocks_of(int V) { return (V + kBlock - 1) / kBlock; }
 
 }  // namespace
 
-// CTAs of a row: enough for six on each SM in all, a block for each warp at least.
+// CTAs of a row: enough for four on each SM in all, a block for each warp at least.
 int token_logprobs_splits(int R, int V, int num_sms) {
   const int most = (blocks_of(V) + kWarps - 1) / kWarps;
-  const long long want = R > 0 ? (6ll * num_sms + R - 1) / R : 1;
+  const long long want = R > 0 ? (4ll * num_sms + R - 1) / R : 1;
   return (int)(want < most ? want : most);
 }
 
@@ -440,7 +592,7 @@ int launch_token_logprobs(const TokenLogprobsArgs& a_in, int splits, void* ws, c
   if (a.V > kMaxLogprobVocab || (long long)a.R * splits > 0x7fffffff) return 1;
   const int n_blocks = blocks_of(a.V);
   a.parts = reinterpret_cast<float*>(ws);
-  a.block_keys = reinterpret_cast<uint32_t*>(a.parts + (size_t)a.R * splits * 4);
+  a.block_max = a.parts + (size_t)a.R * splits * 4;
   if (a.elem == kElemBf16) return launch_one<__nv_bfloat16>(a, splits, n_blocks, s);
   if (a.elem == kElemF16) return launch_one<__half>(a, splits, n_blocks, s);
   return launch_one<float>(a, splits, n_blocks, s);
