@@ -125,14 +125,37 @@ __device__ __forceinline__ void tmem_st16_raw(uint32_t taddr, const uint32_t (&v
       : "memory");
 }
 
+// Halves of the shared-memory matrix descriptors (umma_desc_sw128 and
+// umma_desc_sw128_mn): the low one moves with the address, so that the issuing
+// thread, whose own latency every step passes through, adds one constant per operand.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lbo) {
+  return ((smem_addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
+}
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // SBO, version, 128 B swizzle
+
+// D (TMEM) (+)= A x B, both in shared memory.
+template <bool kAccumulate>
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                        uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %4};\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "n"(kAccumulate ? 1 : 0)
+      : "memory");
+}
+
 // D (TMEM) (+)= A (TMEM, 128 lanes x 16 elements) x B (shared memory).
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
                                         uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(accumulate)
       : "memory");
 }
 
@@ -361,7 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) {
       const uint32_t idesc_s = idesc16<T>(kRows, kKeys, false);
       const uint32_t idesc_pv = idesc16<T>(kRows, D, true);
-      const uint32_t q_base = smem_u32(q_s), k_base = smem_u32(k_s), v_base = smem_u32(v_s);
+      const uint32_t q_lo = desc_lo(smem_u32(q_s), 0), k_lo = desc_lo(smem_u32(k_s), 0),
+                     v_lo = desc_lo(smem_u32(v_s), L::kKvBox);
       int g = 0, it = 0, taken = 0, n = 0;
       bool ok = true;
       auto issue_s = [&](int x, int i) {
@@ -372,13 +396,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    a.status, 241))
           return false;
         tc_fence_after();
-        const uint32_t qa = q_base + x * L::kQTile, ka = k_base + st * L::kKvTile;
+        const uint32_t qa = q_lo + x * (L::kQTile >> 4), ka = k_lo + st * (L::kKvTile >> 4);
+        const uint32_t d = tmem + x * 128 + buf * 64;
+        umma_ss<false>(d, qa, ka, idesc_s);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16(tmem + x * 128 + buf * 64,
-                    umma_desc_sw128(qa + (kk / 4) * L::kQBox + (kk % 4) * 32),
-                    umma_desc_sw128(ka + (kk / 4) * L::kKvBox + (kk % 4) * 32), idesc_s,
-                    kk > 0);
+        for (int kk = 1; kk < D / 16; ++kk)
+          umma_ss<true>(d, qa + (((kk / 4) * L::kQBox + (kk % 4) * 32) >> 4),
+                        ka + (((kk / 4) * L::kKvBox + (kk % 4) * 32) >> 4), idesc_s);
         umma_commit(&s_full[2 * x + buf]);
         if (x == 1) umma_commit(&k_empty[st]);
         if (x == 1 && i == n - 1) umma_commit(q_empty);
@@ -393,12 +417,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i == 0 && it > 0 && !mbar_wait(&o_free[x], (it - 1) & 1, abort_flag, a.status, 244))
           return false;
         tc_fence_after();
-        const uint32_t va = v_base + st * L::kKvTile;
+        const uint32_t va = v_lo + st * (L::kKvTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + buf * 64 + kk * 8,
-                  umma_desc_sw128_mn(va + kk * 2048, L::kKvBox, 1024), idesc_pv,
-                  (i > 0 || kk > 0) ? 1u : 0u);
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + buf * 64 + kk * 8, va + kk * (2048 >> 4),
+                  idesc_pv, kk > 0 ? 1u : (uint32_t)(i > 0));
         umma_commit(&pv_done[2 * x + buf]);
         if (x == 1) umma_commit(&v_empty[st]);
         return true;
