@@ -174,7 +174,9 @@ struct Smem {
   static constexpr int kQBox = kRows * 128;
   static constexpr int kKvTile = kKeys * D * 2;         // K or V of one step
   static constexpr int kKvBox = kKeys * 128;
-  static constexpr int kBytes = 2 * kQTile + 2 * kStages * kKvTile + 1024 /*align*/ + 512;
+  static constexpr int kStage = 32 * 128;               // a warp's output rows, 64 dims
+  static constexpr int kBytes =
+      2 * kQTile + 2 * kStages * kKvTile + 8 * kStage + 1024 /*align*/ + 512;
 };
 
 }  // namespace
@@ -192,7 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* q_s = smem;                                  // row tile X at X * kQTile
   uint8_t* k_s = q_s + 2 * L::kQTile;
   uint8_t* v_s = k_s + kStages * L::kKvTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + kStages * L::kKvTile);
+  uint8_t* o_s = v_s + kStages * L::kKvTile;            // [softmax warp]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(o_s + 8 * L::kStage);
   uint64_t* k_full = bars;                              // [kStages]
   uint64_t* k_empty = k_full + kStages;
   uint64_t* v_full = k_empty + kStages;
@@ -314,42 +317,67 @@ __global__ void __launch_bounds__(kThreads, 1)
                             w.row0 + x * tok1);
             ++qi;
           }
-          const int* table = kPaged ? a.page_table + (size_t)lo * a.table_row : nullptr;
-          for (int i = 0; ok && i < w.steps; ++i, ++g) {
-            const int st = g % kStages;
-            const uint32_t phase = ((g / kStages) - 1) & 1;
-            const int key0 = i * kKeys;
-            // rows past the sequence's end are not fetched (a box at a time)
-            const int boxes = kPaged ? (min(kKeys, len - key0) + box_rows - 1) / box_rows : 1;
-            const uint32_t bytes = L::kBoxes * boxes * box_rows * 128;
-            for (int kv = 0; kv < 2; ++kv) {
-              uint64_t* full = kv == 0 ? &k_full[st] : &v_full[st];
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        // Each lane holds the page and row of one of 32 boxes, and of one of the
+        // next 32: the table's latency is off the loads' path. The copies of a
+        // step go out of as many lanes at once.
+        const int step_boxes = kPaged ? kKeys / box_rows : 1;  // 1, 2 or 4
+        struct Box {
+          int page, row;
+        };
+        auto look_up = [&](int box) {
+          const int key = (box + lane) * box_rows;
+          Box r = {0, 0};
+          if (kPaged && key < len) {
+            r.page = a.page_table[(size_t)lo * a.table_row + key / a.page_size];
+            r.row = kvh * a.page_size + key % a.page_size;
+          }
+          return r;
+        };
+        const int my_box = lane / L::kBoxes, my_col = lane % L::kBoxes;
+        Box held = look_up(0), later = look_up(32);
+        for (int i = 0; i < w.steps && ok; ++i, ++g) {
+          const int st = g % kStages, key0 = i * kKeys;
+          const uint32_t phase = ((g / kStages) - 1) & 1;
+          Box box = {kvh, k0 + key0};  // packed keys: head, first row
+          if (kPaged) {
+            const int first = i * step_boxes;
+            if (i > 0 && first % 32 == 0) {
+              held = later;
+              later = look_up(first + 32);
+            }
+            box.page = __shfl_sync(0xffffffffu, held.page, (first + my_box) & 31);
+            box.row = __shfl_sync(0xffffffffu, held.row, (first + my_box) & 31);
+          }
+          // rows past the sequence's end are not fetched (a box at a time)
+          const int boxes = kPaged ? (min(kKeys, len - key0) + box_rows - 1) / box_rows : 1;
+          if (kPaged && my_box < boxes && my_col == 0 &&
+              (box.page < 0 || box.page >= a.num_pages))  // the copies fill with zeros
+            report_status(a.status, kBoundsViolation, 213);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* full = kv == 0 ? &k_full[st] : &v_full[st];
+            if (lane == 0) {
               if (g >= kStages && !mbar_wait(kv == 0 ? &k_empty[st] : &v_empty[st], phase,
-                                             abort_flag, a.status, 232 + kv)) {
+                                             abort_flag, a.status, 232 + kv))
                 ok = false;
-                break;
-              }
-              uint8_t* dst = (kv == 0 ? k_s : v_s) + st * L::kKvTile;
-              const CUtensorMap* map = kv == 0 ? &tk : &tv;
-              mbar_arrive_expect_tx(full, bytes);
-              if (kPaged) {
-                for (int r = 0; r < boxes; ++r) {
-                  const int key = key0 + r * box_rows;
-                  const int page = table[key / a.page_size];
-                  if (page < 0 || page >= a.num_pages)  // the copy fills with zeros
-                    report_status(a.status, kBoundsViolation, 213);
-                  for (int c = 0; c < L::kBoxes; ++c)
-                    tma_load_3d(dst + c * L::kKvBox + r * box_rows * 128, map, full, c * 64,
-                                kvh * a.page_size + key % a.page_size, page);
-                }
-              } else {
-                for (int c = 0; c < L::kBoxes; ++c)
-                  tma_load_3d(dst + c * L::kKvBox, map, full, c * 64, kvh, k0 + key0);
-              }
+              else
+                mbar_arrive_expect_tx(full, L::kBoxes * boxes * box_rows * 128);
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (!ok) break;
+            uint8_t* dst = (kv == 0 ? k_s : v_s) + st * L::kKvTile + my_col * L::kKvBox;
+            const CUtensorMap* map = kv == 0 ? &tk : &tv;
+            if (my_box < boxes) {
+              if (kPaged)
+                tma_load_3d(dst + my_box * box_rows * 128, map, full, my_col * 64, box.row,
+                            box.page);
+              else
+                tma_load_3d(dst, map, full, my_col * 64, box.page, box.row);
             }
           }
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
       // the next item; with the last fetch of the launch the counter is zero again
       if (lane == 0) item = (int)gridDim.x + (int)atomicInc(
@@ -560,36 +588,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[2 * x + buf]);
       }
       if (!ok) break;
-      const bool valid = has_token && tok < w.tokens;
-      T* dst = reinterpret_cast<T*>(a.out) +
-               ((size_t)(w.row0 + tok) * a.nq + w.kvh * G + row % G) * D;
       const float l = l2.x + l2.y;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = 1.f / l;
       if (w.steps > 0) {
         if (!wait_all(&pv_done[2 * x + ((g - 1) & 1)], ((g - 1) >> 1) & 1, 254)) break;
         tc_fence_after();
       }
+      // 64 dims at a time through shared memory, so that a store instruction
+      // covers whole 128-byte lines of four rows (a row a lane took 4100 cycles)
+      uint8_t* stage = o_s + (warp - 2) * L::kStage;
+      T* out = reinterpret_cast<T*>(a.out) +
+               ((size_t)(w.row0 + x * tok1) * a.nq + w.kvh * G) * D + lane % 8 * 8;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
+      for (int c = 0; c < D / 64; ++c) {
+        float o[64];
         if (w.steps > 0) {
-          tmem_ld32(t_o + c * 32, o);
+          tmem_ld64(t_o + c * 64, o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          for (int e = 0; e < 64; ++e) o[e] = 0.f;
         }
-        if (valid) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 v;
-            // a row that saw no key: exact zeros whatever O holds
-            v.x = l > 0.f ? pack2<T>(o[8 * e + 0] * inv, o[8 * e + 1] * inv) : 0u;
-            v.y = l > 0.f ? pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv) : 0u;
-            v.z = l > 0.f ? pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv) : 0u;
-            v.w = l > 0.f ? pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv) : 0u;
-            *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = v;
-          }
+        for (int u = 0; u < 8; ++u) {
+          uint4 v;
+          // a row that saw no key: exact zeros whatever O holds
+          v.x = l == 0.f ? 0u : pack2<T>(o[8 * u + 0] * inv, o[8 * u + 1] * inv);
+          v.y = l == 0.f ? 0u : pack2<T>(o[8 * u + 2] * inv, o[8 * u + 3] * inv);
+          v.z = l == 0.f ? 0u : pack2<T>(o[8 * u + 4] * inv, o[8 * u + 5] * inv);
+          v.w = l == 0.f ? 0u : pack2<T>(o[8 * u + 6] * inv, o[8 * u + 7] * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = v;
         }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rw = k * 4 + lane / 8, r = qq * 32 + rw, t = r / G;
+          if (r < tok1 * G && x * tok1 + t < w.tokens)
+            *reinterpret_cast<uint4*>(out + ((size_t)t * a.nq + (r - t * G)) * D + c * 64) =
+                *reinterpret_cast<const uint4*>(stage + rw * 128 + ((lane % 8 ^ (rw & 7)) << 4));
+        }
+        __syncwarp();
       }
       if (w.steps > 0) {
         tc_fence_before();
