@@ -223,6 +223,14 @@ class DisaggregatedQwenModel:
                           timeout_ms=timeout_ms)
         return m
 
+    def ragged(self, num_pages: int, page_size: int = 64):
+        """A ``RaggedGenerator`` (prompts of different lengths over a paged cache) on
+        this process's workers; both roles have to live here."""
+        from .ragged import RaggedGenerator
+        if not (self.ctx.is_attention_node and self.ctx.is_ffn_node):
+            raise NotImplementedError("ragged batches run where both roles live (one process)")
+        return RaggedGenerator(self.attention_worker, self.ffn_worker, num_pages, page_size)
+
     # ----------------------------------------------------------- forwards
     def plan(self, global_batch: int, q_len: int, num_micro_batches: int) -> ForwardPlan:
         return make_plan(self.topology, global_batch, num_micro_batches, q_len)
