@@ -28,11 +28,13 @@
 //
 // Split: the 16-key blocks of all (sequence, kv head) items, in order, are cut
 // into equal ranges, one per CTA, whatever the lengths: the last CTA ends when the
-// first does. A CTA joins its 8 warps in shared memory; an item cut by a range
+// first does. A CTA joins its 4 warps in shared memory; an item cut by a range
 // end leaves fp32 partials (O, maximum, sum) in the workspace, and the CTA
 // that counts the last of its parts joins them, in the order of the parts.
 
 #include <string.h>
+
+#include <atomic>
 
 #include "ragged.cuh"
 
@@ -653,9 +655,17 @@ static int launch_one(const PagedDecodeArgs& a, int grid, int groups, const CUte
                       const CUtensorMap& tv, cudaStream_t s) {
   const auto kern = paged_decode_kernel<T, D, NT>;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), Dec<D>::kBytes);
-  if (e == cudaSuccess)  // room for both CTAs of an SM
+  int dev = 0;
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return 4000 + (int)e;
+  // room for both CTAs of an SM, asked for once per device
+  static std::atomic<uint64_t> asked{0};
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(asked.load(std::memory_order_relaxed) & bit)) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  }
   if (e == cudaSuccess)
     e = launch_k(kern, dim3(grid), dim3(kThreads), Dec<D>::kBytes, s, tk, tv, a, groups);
   return e == cudaSuccess ? 0 : 4000 + (int)e;
