@@ -66,7 +66,7 @@ at::Tensor zeroed_counters(const at::Tensor& like, int64_t n) {
 }
 
 // Workspace that no call expects anything in: one buffer for each stream, which
-// grows (at most 10 MB: the split forms of few rows alone use it) and is kept,
+// grows (at most about 40 MB: the split forms of few rows alone use it) and is kept,
 // 0.8 us less on the host than an allocation a call. A capture gets its own.
 at::Tensor scratch(const at::Tensor& like, int64_t bytes) {
   const auto opt = at::TensorOptions().device(like.device()).dtype(at::kByte);
@@ -219,6 +219,18 @@ at::Tensor packed_common(PackedAttnArgs& a, const at::Tensor& q, const at::Tenso
   return out;
 }
 
+void run_packed(PackedAttnArgs& a, const at::Tensor& q, int64_t most_keys, const char* what) {
+  const int sms = num_sms();
+  const at::Tensor counter = zeroed_counters(q, 1);
+  a.counter = counter.data_ptr<int>();
+  a.splits = packed_attention_splits(a.T, a.n_seqs, a.nq, a.nkv, most_keys, sms);
+  at::Tensor parts;
+  if (a.splits > 1)
+    parts = scratch(q, packed_attention_part_bytes((int64_t)a.T * a.nq, a.D, a.splits));
+  check_rc(launch_packed_attention(a, a.splits > 1 ? parts.data_ptr() : nullptr, sms, stream()),
+           what);
+}
+
 at::Tensor packed_attention(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
                             const at::Tensor& cu_q, const OptTensor& cu_k_in,
                             c10::optional<double> scale, const OptTensor& status) {
@@ -241,9 +253,7 @@ at::Tensor packed_attention(const at::Tensor& q_in, const at::Tensor& k_in, cons
   a.v_row = v.stride(0);
   a.Tk = (int)k.size(0);
   a.cu_k = cu_k.data_ptr<int>();
-  const at::Tensor counter = zeroed_counters(q, 1);
-  a.counter = counter.data_ptr<int>();
-  check_rc(launch_packed_attention(a, num_sms(), stream()), "packed_attention");
+  run_packed(a, q, a.Tk, "packed_attention");
   return out;
 }
 
@@ -264,9 +274,7 @@ at::Tensor paged_prefill_attention(const at::Tensor& q_in, const at::Tensor& k_p
   a.k_pages = k_pages.data_ptr();
   a.v_pages = v_pages.data_ptr();
   a.seq_lens = seq_lens.data_ptr<int>();
-  const at::Tensor counter = zeroed_counters(q, 1);
-  a.counter = counter.data_ptr<int>();
-  check_rc(launch_packed_attention(a, num_sms(), stream()), "paged_prefill_attention");
+  run_packed(a, q, (int64_t)a.max_pages * a.page_size, "paged_prefill_attention");
   return out;
 }
 

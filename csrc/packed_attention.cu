@@ -13,10 +13,9 @@
 //
 // Steps of 64 keys. For row tile X, S_X = Q_X K^T (M 128, N 64) and
 // O_X += P_X V (P from TMEM) accumulate in TMEM; S and P of consecutive steps
-// take two buffers in turn, so the product S_X(i+1) is finished while the
-// softmax of step i still runs and the softmax warps never wait for the tensor
-// core's latency. With one buffer (S of 128 keys, P over it) that chain
-// softmax -> P V -> S bounded the step.
+// take two buffers in turn, so the product S_X(i+1) runs beside the softmax of
+// step i. With one buffer (S freed once the softmax holds it, P apart) the four
+// long prompts below took 927 us.
 //
 //   warp 0      work items, TMA producer: Q tiles, then K and V rings of 4 steps
 //   warp 1      TMEM owner (512 columns) and MMA issuer
@@ -39,8 +38,26 @@
 // blocks belongs to the last sequence i with cu[i] / TB + i <= s: that leaves
 // at least ceil(length / TB) slots for each sequence without a prefix sum over
 // lengths, and a sequence's longest-running blocks come first.
+//
+// Where the blocks are too few for the SMs (a chunk of few tokens over a long
+// cache), the keys of a block are cut into equal parts, as many as fill the SMs
+// once, of 8 steps at least; each part leaves O, maximum and sum in fp32 and a
+// second kernel joins the rows. 4 chunks of 16 tokens over 20000 positions: 45 us
+// split, 260 whole; parts of 6 steps at least do no better, of 12 worse (4 x 16
+// over 2000: 24 us, 18.5 with 8).
+//
+// Measured (bf16, 32 heads over 4 of 128): 4 prompts of 2338..8192 tokens, 991
+// GFLOP visible, 840..880 us, 1.13..1.18 PF/s; 32 prompts of 5..1021, 72 us. A step of both
+// row tiles takes 1.06 us: 0.75 of MMAs at the GEMM's measured rate, and 0.55 of
+// exponentials beside them. What keeps the tensor cores from their rate is shared
+// memory: with 64 keys, S's MMA reads 6 KB (48 cycles) for 32 cycles of products,
+// so a step's reads and the arriving tiles take 1280 cycles of it. One row tile
+// a CTA, two CTAs an SM, has the tiles arrive twice: 940 us, though 68 us for the
+// 32 prompts, whose 5 steps a block hide less of each block's start and end.
 
 #include <string.h>
+
+#include <algorithm>
 
 #include "ragged.cuh"
 
@@ -53,11 +70,16 @@ constexpr int kKeys = 64;     // keys of a step
 constexpr int kStages = 4;    // K and V ring depth
 constexpr int kThreads = 320;
 
+// Parts of an item's keys: at most kMaxParts, of kMinPart steps at least.
+constexpr int kMaxParts = 32;
+constexpr int kMinPart = 8;
+
 struct Item {
-  int steps;    // 64-key steps; 0: no key; -1: no more work
+  int steps;    // 64-key steps of this part; 0: no key; -1: no more work
+  int parts;    // number of parts | this one << 8
   int row0;     // query row of the block's first token
   int tokens;   // tokens of the sequence from there on (may exceed the block)
-  int pos0;     // position of the first token
+  int pos0;     // position of the first token, from the part's first key on
   int kvh;
 };
 
@@ -260,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int item = blockIdx.x;
     while (item < n_items) {
-      const int slot = item / a.nkv, kvh = item % a.nkv;
+      const int unit = a.splits > 1 ? item / a.splits : item, part = item - unit * a.splits;
+      const int slot = unit / a.nkv, kvh = unit % a.nkv;
       // the last sequence whose first slot is at or before `slot`; sequence
       // n_seqs stands for the rows past the last offset
       int lo = 0, hi = a.n_seqs + 1;
@@ -275,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.kvh = kvh;
       const int q0 = cu_q(lo), q1 = lo < a.n_seqs ? max(cu_q(lo + 1), q0) : a.T;
       const int blocks = (q1 - q0 + block_tokens - 1) / block_tokens;
-      const int block = blocks - 1 - (slot - (q0 / block_tokens + lo));
+      int block = blocks - 1 - (slot - (q0 / block_tokens + lo));
       int k0 = 0, len = 0;
       if (lo < a.n_seqs && block >= 0) {
         if (lane == 0 && (a.cu_q[lo] != q0 || a.cu_q[lo + 1] != q1))
@@ -294,7 +317,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       w.tokens = q1 - w.row0;
       w.pos0 = len - (q1 - w.row0);
       const int last = len > 0 ? w.pos0 + min(w.tokens, block_tokens) - 1 : -1;
-      w.steps = last >= 0 ? last / kKeys + 1 : 0;
+      const int steps = last >= 0 ? last / kKeys + 1 : 0;
+      int first_key = 0;
+      w.steps = steps;
+      w.parts = 1;
+      if (a.splits > 1) {
+        const int parts = min(max(steps / kMinPart, 1), a.splits);
+        const int first_step = steps * part / parts;
+        w.steps = steps * (part + 1) / parts - first_step;
+        w.parts = parts | part << 8;
+        first_key = first_step * kKeys;
+        w.pos0 -= first_key;
+        if (part >= parts) block = -1;
+      }
       if (block >= 0 && ok) {
         // hand the item to the other warps
         const int ib = published & 1;
@@ -327,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int page, row;
         };
         auto look_up = [&](int box) {
-          const int key = (box + lane) * box_rows;
+          const int key = first_key + (box + lane) * box_rows;
           Box r = {0, 0};
           if (kPaged && key < len) {
             r.page = a.page_table[(size_t)lo * a.table_row + key / a.page_size];
@@ -338,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int my_box = lane / L::kBoxes, my_col = lane % L::kBoxes;
         Box held = look_up(0), later = look_up(32);
         for (int i = 0; i < w.steps && ok; ++i, ++g) {
-          const int st = g % kStages, key0 = i * kKeys;
+          const int st = g % kStages, key0 = first_key + i * kKeys;
           const uint32_t phase = ((g / kStages) - 1) & 1;
           Box box = {kvh, k0 + key0};  // packed keys: head, first row
           if (kPaged) {
@@ -594,40 +629,59 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait_all(&pv_done[2 * x + ((g - 1) & 1)], ((g - 1) >> 1) & 1, 254)) break;
         tc_fence_after();
       }
-      // 64 dims at a time through shared memory, so that a store instruction
-      // covers whole 128-byte lines of four rows (a row a lane took 4100 cycles)
-      uint8_t* stage = o_s + (warp - 2) * L::kStage;
-      T* out = reinterpret_cast<T*>(a.out) +
-               ((size_t)(w.row0 + x * tok1) * a.nq + w.kvh * G) * D + lane % 8 * 8;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        float o[64];
-        if (w.steps > 0) {
-          tmem_ld64(t_o + c * 64, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) o[e] = 0.f;
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          uint4 v;
-          // a row that saw no key: exact zeros whatever O holds
-          v.x = l == 0.f ? 0u : pack2<T>(o[8 * u + 0] * inv, o[8 * u + 1] * inv);
-          v.y = l == 0.f ? 0u : pack2<T>(o[8 * u + 2] * inv, o[8 * u + 3] * inv);
-          v.z = l == 0.f ? 0u : pack2<T>(o[8 * u + 4] * inv, o[8 * u + 5] * inv);
-          v.w = l == 0.f ? 0u : pack2<T>(o[8 * u + 6] * inv, o[8 * u + 7] * inv);
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = v;
-        }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int rw = k * 4 + lane / 8, r = qq * 32 + rw, t = r / G;
-          if (r < tok1 * G && x * tok1 + t < w.tokens)
-            *reinterpret_cast<uint4*>(out + ((size_t)t * a.nq + (r - t * G)) * D + c * 64) =
-                *reinterpret_cast<const uint4*>(stage + rw * 128 + ((lane % 8 ^ (rw & 7)) << 4));
-        }
-        __syncwarp();
+      if (a.splits > 1 && has_token && tok < w.tokens) {
+        const size_t r = (size_t)(w.row0 + tok) * a.nq + w.kvh * G + row % G;
+        if (w.parts < 256) a.n_parts[r] = w.parts;
+        a.part_ml[(size_t)(w.parts >> 8) * a.T * a.nq + r] = make_float2(m, l);
       }
+      // Through shared memory, so that a store instruction covers whole 128-byte
+      // lines of four rows (a row a lane took 4100 cycles for an item's rows).
+      // `Out` is the output's type, or float for a part's O as it is.
+      auto store = [&](auto* base, auto kind) {
+        using Out = decltype(kind);
+        constexpr int kDims = 128 / sizeof(Out);
+        uint8_t* stage = o_s + (warp - 2) * L::kStage;
+        Out* out = reinterpret_cast<Out*>(base) +
+                   ((size_t)(w.row0 + x * tok1) * a.nq + w.kvh * G) * D + lane % 8 * (kDims / 8);
+#pragma unroll
+        for (int c = 0; c < D / kDims; ++c) {
+          float o[kDims];
+          if (w.steps > 0) {
+            if constexpr (kDims == 64) tmem_ld64(t_o + c * 64, o);
+            else tmem_ld32(t_o + c * 32, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) o[e] = 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            uint4 v;
+            // a row that saw no key: exact zeros whatever O holds
+            if constexpr (kDims == 64) {
+              v.x = l == 0.f ? 0u : pack2<T>(o[8 * u + 0] * inv, o[8 * u + 1] * inv);
+              v.y = l == 0.f ? 0u : pack2<T>(o[8 * u + 2] * inv, o[8 * u + 3] * inv);
+              v.z = l == 0.f ? 0u : pack2<T>(o[8 * u + 4] * inv, o[8 * u + 5] * inv);
+              v.w = l == 0.f ? 0u : pack2<T>(o[8 * u + 6] * inv, o[8 * u + 7] * inv);
+            } else {
+              v = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]),
+                             __float_as_uint(o[4 * u + 2]), __float_as_uint(o[4 * u + 3]));
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = v;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rw = k * 4 + lane / 8, r = qq * 32 + rw, t = r / G;
+            if (r < tok1 * G && x * tok1 + t < w.tokens)
+              *reinterpret_cast<uint4*>(out + ((size_t)t * a.nq + (r - t * G)) * D + c * kDims) =
+                  *reinterpret_cast<const uint4*>(stage + rw * 128 +
+                                                  ((lane % 8 ^ (rw & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      };
+      if (w.parts != 1) store(a.part_o + (size_t)(w.parts >> 8) * a.T * a.nq * D, float());
+      else store(a.out, T());
       if (w.steps > 0) {
         tc_fence_before();
         __syncwarp();
@@ -644,7 +698,55 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Joins the parts of the rows that have several, D / 4 threads a row:
+//   out = sum_p w_p O_p / sum_p w_p l_p,  w_p = 2^(m_p - max m)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_parts_kernel(PackedAttnArgs a) {
+  constexpr int kLanes = D / 4;
+  pdl_wait();
+  pdl_trigger();
+  const size_t rows = (size_t)a.T * a.nq;
+  const size_t r = ((size_t)blockIdx.x * 128 + threadIdx.x) / kLanes;
+  if (r >= rows) return;
+  const int parts = min(a.n_parts[r], a.splits);
+  if (parts <= 1) return;
+  float most = -INFINITY;
+  for (int p = 0; p < parts; ++p) most = fmaxf(most, a.part_ml[p * rows + r].x);
+  const int at = threadIdx.x % kLanes * 4;
+  float l = 0.f, o[4] = {};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = a.part_ml[p * rows + r];
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * rows + r) * D + at);
+    if (ml.y == 0.f) continue;  // the row saw none of the part's keys
+    const float w = exp2_approx(ml.x - most);
+    l = fmaf(w, ml.y, l);
+    o[0] = fmaf(w, v.x, o[0]);
+    o[1] = fmaf(w, v.y, o[1]);
+    o[2] = fmaf(w, v.z, o[2]);
+    o[3] = fmaf(w, v.w, o[3]);
+  }
+  const float inv = 1.f / l;
+  uint2 v = make_uint2(0u, 0u);
+  if (l != 0.f) v = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + r * D + at) = v;
+}
+
 // ============================================================ host side ===
+
+int packed_attention_splits(long long T, int n_seqs, int nq, int nkv, long long most_keys,
+                            int num_sms) {
+  const int block = 2 * (kRows / (nq / nkv));
+  const long long blocks = T / block + n_seqs / 2;  // about: a last block of each is half full
+  const long long items = (blocks > 0 ? blocks : 1) * nkv;
+  const long long s =
+      std::min((num_sms + items / 4) / items, most_keys / (kMinPart * kKeys));
+  return (int)std::min<long long>(std::max<long long>(s, 1), kMaxParts);
+}
+
+long long packed_attention_part_bytes(long long rows, int D, int splits) {
+  return splits > 1 ? rows * (4 + (8 + 4ll * D) * splits) + 32 : 0;
+}
 
 template <typename T, int D, bool kPaged>
 static int launch_one(const PackedAttnArgs& a, int num_sms, const CUtensorMap& tq,
@@ -653,16 +755,30 @@ static int launch_one(const PackedAttnArgs& a, int num_sms, const CUtensorMap& t
   const auto kern = packed_attention_kernel<T, D, kPaged>;
   cudaError_t e = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
   if (e != cudaSuccess) return 4000 + (int)e;
-  const long long items = ((long long)a.T / (2 * tok1) + a.n_seqs + 1) * a.nkv;
+  const long long items = ((long long)a.T / (2 * tok1) + a.n_seqs + 1) * a.nkv * a.splits;
   if (items > 0x3fffffff) return 1;
   const int grid = (int)(items < num_sms ? items : num_sms);
   e = launch_k(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, s, tq, tk, tv, a, tok1,
                (int)items, box_rows);
+  if (e == cudaSuccess && a.splits > 1) {
+    const long long threads = (long long)a.T * a.nq * (D / 4);
+    e = launch_k(join_parts_kernel<T, D>, dim3((unsigned)((threads + 127) / 128)), dim3(128), 0, s,
+                 a);
+  }
   return e == cudaSuccess ? 0 : 4000 + (int)e;
 }
 
-int launch_packed_attention(const PackedAttnArgs& a, int num_sms, cudaStream_t s) {
+int launch_packed_attention(const PackedAttnArgs& a_in, void* parts, int num_sms,
+                            cudaStream_t s) {
+  PackedAttnArgs a = a_in;
   if (a.T == 0) return 0;
+  {  // O (16-byte aligned), then (m, l), then the numbers of parts
+    const long long rows = (long long)a.T * a.nq;
+    if (a.splits < 1 || a.splits > kMaxParts || rows * (a.D / 4) / 128 >= 0x7fffffff) return 1;
+    a.part_o = reinterpret_cast<float*>(parts);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * a.D * a.splits);
+    a.n_parts = reinterpret_cast<int*>(a.part_ml + rows * a.splits);
+  }
   if (!a.paged && a.Tk == 0) {  // no key anywhere
     const cudaError_t e = cudaMemsetAsync(a.out, 0, (size_t)a.T * a.nq * a.D * 2, s);
     return e == cudaSuccess ? 0 : 4000 + (int)e;

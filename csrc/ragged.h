@@ -77,8 +77,16 @@ struct PackedAttnArgs {
   int elem;
   int* status;
   int* counter;             // [1], zero; left zero
+  int splits;               // parts of a block's keys at most; 1: none is split
+  float* part_o;            // filled in by the launch: O [splits, T, nq, D],
+  float2* part_ml;          // maximum and sum [splits, T, nq],
+  int* n_parts;             // parts [T, nq]
 };
-int launch_packed_attention(const PackedAttnArgs& a, int num_sms, cudaStream_t s);
+// Parts that fill the GPU where there are few blocks, for keys up to most_keys.
+int packed_attention_splits(long long T, int n_seqs, int nq, int nkv, long long most_keys,
+                            int num_sms);
+long long packed_attention_part_bytes(long long rows, int D, int splits);
+int launch_packed_attention(const PackedAttnArgs& a, void* parts, int num_sms, cudaStream_t s);
 
 // Per-head RMSNorm and RoPE of the q and k heads of a packed qkv projection.
 // q goes to q_out; k to k_out [T, nkv, D], or with the pool given, k and v to

@@ -346,6 +346,59 @@ def test_paged_prefill_bad_indices_are_recorded():
     _close(out[10:], _exact_rows(q[10:], k, v), torch.bfloat16)
 
 
+@pytest.mark.parametrize("nq,nkv,D", [(32, 4, 128), (16, 2, 64), (3, 1, 128), (40, 1, 128), (8, 8, 64)])
+@pytest.mark.parametrize("news,total", [
+    ([16], [20011]), ([1], [1024]), ([1], [1023]), ([1, 16, 5, 0], [20000, 4097, 1087, 700]),
+    ([40, 3], [8200, 0]), ([130], [5000]), ([9, 0, 1, 1], [512, 0, 1, 64])])
+def test_paged_prefill_few_tokens_over_long_caches(nq, nkv, D, news, total):
+    """The keys are split over CTAs and the parts joined."""
+    for dtype in DTYPES:
+        g = _gen(sum(total))
+        kp, vp, table, dense = _pool(g, total, nkv, D, 64, dtype)
+        q = _randn(g, sum(news), nq, D, dtype=dtype, scale=2.0)
+        status = torch.zeros(2, dtype=torch.int32, device=DEV)
+        args = (q, kp, vp, table, _i32(total), _cu(news))
+        out = ops.paged_prefill_attention(*args, status=status)
+        a = 0
+        for n, (k, v) in zip(news, dense):
+            if k.shape[0] == 0:
+                assert not out[a:a + n].any()
+            else:
+                _close(out[a:a + n], _exact_rows(q[a:a + n], k, v), dtype)
+            a += n
+        assert status.tolist()[0] == 0
+        assert torch.equal(out, ops.paged_prefill_attention(*args))  # same bits
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_attention_split_keys_rows_without_any(D):
+    """Queries before the first key, and rows past the last offset, in a call
+    whose keys are split; a part's keys may all lie after a row's position."""
+    g = _gen(D)
+    q_lens, k_lens = [70, 30], [2100, 20]
+    q = _randn(g, 110, 4, D, scale=2.0)
+    k, v = _randn(g, 2120, 2, D), _randn(g, 2120, 2, D)
+    out = ops.packed_attention(q, k, v, _cu(q_lens), _cu(k_lens))
+    _close(out[:70], _exact_rows(q[:70], k[:2100], v[:2100]), torch.bfloat16)
+    assert not out[70:80].any() and not out[100:].any()
+    _close(out[80:100], _exact_rows(q[80:100], k[2100:], v[2100:]), torch.bfloat16)
+
+
+def test_paged_prefill_split_replays_with_other_lengths():
+    """One captured call, replayed as the cache grows from no split to many parts."""
+    g = _gen(21)
+    kp, vp, table, dense = _pool(g, [9000], 4, 128, 64, torch.bfloat16)
+    q, cu, seq = _randn(g, 8, 32, 128), _i32([0, 8]), _i32([9000])
+    ops.paged_prefill_attention(q, kp, vp, table, seq, cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill_attention(q, kp, vp, table, seq, cu)
+    for n in (9000, 8, 600, 1100, 64, 8999):
+        seq.fill_(n)
+        graph.replay()
+        _close(out, _exact_rows(q, *(x[:n] for x in dense[0])), torch.bfloat16)
+
+
 # ----------------------------------------------------------------- norm + RoPE --
 def _exact_norm_rope(x, w, cs, eps):
     D = x.shape[-1]
