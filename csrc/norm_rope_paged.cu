@@ -13,6 +13,10 @@
 // head, each with two runs of 8 elements (16 bytes) that RoPE pairs, and keep
 // the loads of kHeads heads of their token on the way at once; the table's
 // row and the page slot, of the token, come with them.
+//
+// Measured (8191 tokens, 32 + 4 heads of 128, bf16, 172 MB read and written):
+// 37 us, 4.6 TB/s. One head at a time 41.6, four in blocks of 256 threads 44,
+// a head a thread block with 2-byte loads 130.
 
 #include "ragged.cuh"
 

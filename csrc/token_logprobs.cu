@@ -24,6 +24,9 @@
 // blocks, reads them again (k KB, from L2) and ranks the few elements that reach
 // the smallest of the picked maxima.
 //
+// Measured (4096 rows of 151936, bf16, top 8; 1245 MB): 213 us, 5.8 TB/s. Blocks
+// loaded to registers one ahead took 323, the ring with the maxima in fp32 250.
+//
 // Few rows are split over several CTAs: each leaves (m, Z, S) and its block
 // maxima in the workspace, and the CTA that counts the row's last part
 // finishes the row.
