@@ -297,39 +297,43 @@ __device__ int list_top(Shared<T>& sh, const T* x, int V, int n_blocks, int top_
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (warp == 0) {
     // top_k rounds: the largest key left, the first block of equals. The lanes
-    // hold the keys of up to 512 blocks in registers.
+    // hold the keys of up to 512 blocks in registers, neighbours in a lane, so that
+    // the first lane with the key has the first block.
     const int n = min(top_k, n_blocks);
-    const bool held = n_blocks <= 32 * 16;
-    uint32_t key[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      key[i] = held && i * 32 + lane < n_blocks ? sh.keys[i * 32 + lane] : 0;
     uint32_t k = 0;
-    for (int r = 0; r < n; ++r) {
-      uint32_t best = 0;
-      if (held) {
+    if (n_blocks <= 32 * 16) {
+      const int per = (n_blocks + 31) / 32;
+      uint32_t key[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) best = max(best, key[i]);
-      } else {
+      for (int i = 0; i < 16; ++i)
+        key[i] = i < per && lane * per + i < n_blocks ? sh.keys[lane * per + i] : 0;
+      for (int r = 0; r < n; ++r) {
+        uint32_t m[4] = {key[0], key[1], key[2], key[3]};
+#pragma unroll
+        for (int i = 4; i < 16; ++i) m[i % 4] = max(m[i % 4], key[i]);
+        const uint32_t best = max(max(m[0], m[1]), max(m[2], m[3]));
+        uint32_t at[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) at[i % 4] |= key[i] == best ? 1u << i : 0u;
+        const int first = __ffs((at[0] | at[1]) | (at[2] | at[3])) - 1;
+        k = __reduce_max_sync(0xffffffffu, best);
+        const int who = __ffs(__ballot_sync(0xffffffffu, best == k)) - 1;
+        if (lane == who) sh.sel[r] = lane * per + first;
+        const int gone = lane == who ? first : -1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) key[i] = i == gone ? 0u : key[i];
+      }
+    } else {
+      for (int r = 0; r < n; ++r) {
+        uint32_t best = 0;
         for (int i = lane; i < n_blocks; i += 32) best = max(best, sh.keys[i]);
-      }
-      k = __reduce_max_sync(0xffffffffu, best);
-      unsigned at = 0xffffffffu;
-      if (held) {
-#pragma unroll
-        for (int i = 15; i >= 0; --i)
-          if (key[i] == k) at = i * 32 + lane;
-      } else if (best == k) {
-        for (int i = n_blocks - 1; i >= 0; --i)
-          if (i % 32 == lane && sh.keys[i] == k) at = i;
-      }
-      const int b = (int)__reduce_min_sync(0xffffffffu, at);
-      if (lane == 0) sh.sel[r] = b;
-      if (held) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i * 32 + lane == b) key[i] = 0;
-      } else {
+        k = __reduce_max_sync(0xffffffffu, best);
+        unsigned at = 0xffffffffu;
+        if (best == k)
+          for (int i = n_blocks - 1; i >= 0; --i)
+            if (i % 32 == lane && sh.keys[i] == k) at = i;
+        const int b = (int)__reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) sh.sel[r] = b;
         if (b % 32 == lane) sh.keys[b] = 0;
         __syncwarp();
       }
@@ -578,11 +582,15 @@ int blocks_of(int V) { return (V + kBlock - 1) / kBlock; }
 
 }  // namespace
 
-// CTAs of a row: enough for four on each SM in all, a block for each warp at least.
+// CTAs of a row: two on each SM in all at most, a block for each warp at least
+// (33 rows of fp32, top 20: 17.0 us with 8 CTAs a row, 18.2 with 17; 256 of bf16: 29 with
+// one, 35 with two to four). Between two and four rows an SM, where one CTA a row
+// leaves the last ones alone, two: 400 rows 45 us, 52 with one.
 int token_logprobs_splits(int R, int V, int num_sms) {
   const int most = (blocks_of(V) + kWarps - 1) / kWarps;
-  const long long want = R > 0 ? (4ll * num_sms + R - 1) / R : 1;
-  return (int)(want < most ? want : most);
+  int want = 2 * num_sms / max(R, 1);
+  if (want < 1) want = R < 4 * num_sms ? 2 : 1;
+  return want < most ? want : most;
 }
 
 long long token_logprobs_workspace(int R, int V, int splits) {
