@@ -47,13 +47,14 @@
 // over 2000: 24 us, 18.5 with 8).
 //
 // Measured (bf16, 32 heads over 4 of 128): 4 prompts of 2338..8192 tokens, 991
-// GFLOP visible, 840..880 us, 1.13..1.18 PF/s; 32 prompts of 5..1021, 72 us. A step of both
-// row tiles takes 1.06 us: 0.75 of MMAs at the GEMM's measured rate, and 0.55 of
-// exponentials beside them. What keeps the tensor cores from their rate is shared
-// memory: with 64 keys, S's MMA reads 6 KB (48 cycles) for 32 cycles of products,
-// so a step's reads and the arriving tiles take 1280 cycles of it. One row tile
-// a CTA, two CTAs an SM, has the tiles arrive twice: 940 us, though 68 us for the
-// 32 prompts, whose 5 steps a block hide less of each block's start and end.
+// GFLOP visible, 865 us, 1.15 PF/s; 32 prompts of 5..1021, 72 us. A step of both row
+// tiles takes 1820 cycles, for 1024 of products and as many of exponentials (4096
+// tokens: tensor pipe 57%, special function units 61%, issue slots 40%, reads of
+// shared memory by the MMAs 57%): none is full, what is left is the chain of a
+// tile's softmax, P V, and S two steps on, between the two tiles. Other orders of the
+// MMAs (S_X(i+2) right behind P_X(i) V; S before P V) take 970..1030 us. One row tile a
+// CTA, two CTAs an SM, takes 940 us, and 68 for the 32 prompts, whose 5 steps a block
+// hide less of each block's start and end.
 
 #include <string.h>
 
