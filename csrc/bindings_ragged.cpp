@@ -152,7 +152,10 @@ void take_table(Args& a, const at::Tensor& table, int64_t n, const at::Tensor& l
                   table.dim() == 2 && table.size(0) == n && table.size(1) >= 1 &&
                   (n == 0 || table.size(1) == 1 || table.stride(1) == 1),
               "page_table must be an int32 [", std::to_string(n), ", pages] on the same device with unit stride");
-  TORCH_CHECK_VALUE(table.size(1) * a.page_size < (1ll << 31), "page_table spans too many positions");
+  // positions are ints, and the kernels look a few thousand ahead of the last one
+  TORCH_CHECK_VALUE(table.size(1) * a.page_size < (1ll << 30) &&
+                        (n <= 1 || table.stride(0) < (1ll << 31)),
+                    "page_table spans too many positions");
   a.page_table = table.data_ptr<int>();
   a.table_row = (int)table.stride(0);
   a.max_pages = (int)table.size(1);

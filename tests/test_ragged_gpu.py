@@ -608,3 +608,18 @@ def test_refusals():
                    (6, pos.long()), (7, slots.int()), (8, 5)):
         with pytest.raises(ValueError):
             ops.qk_norm_rope_paged(*[bad if j == i else a for j, a in enumerate(args)])
+
+
+def test_page_tables_past_the_positions_of_an_int_are_refused():
+    q = torch.zeros(1, 1, 64, device=DEV, dtype=torch.half)
+    pages = torch.zeros(1, 1, 4096, 64, device=DEV, dtype=torch.half)
+    for columns, fits in ((2 ** 18 - 1, True), (2 ** 18, False)):
+        table = torch.zeros(1, columns, dtype=torch.int32, device=DEV)
+        for call in (lambda t: ops.paged_decode_attention(q, pages, pages, t, _i32([5000])),
+                     lambda t: ops.paged_prefill_attention(q, pages, pages, t, _i32([5000]),
+                                                           _i32([0, 1]))):
+            if fits:
+                assert not call(table).any()
+            else:
+                with pytest.raises(ValueError):
+                    call(table)
