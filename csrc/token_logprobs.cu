@@ -12,8 +12,8 @@
 // What bounds it is reading the logits once. A warp takes blocks of 512
 // elements, the next block on its way while one is summed: the block's maximum
 // by one warp reduction (a running maximum of the warp's, so that sums are
-// rescaled only when it moves), then an exponential, two multiply-adds and an add
-// per element, in pairs. The loop issues about 100 instructions for a block's 16
+// rescaled only when it moves), then a subtraction, a product, an exponential, an add
+// and a multiply-add per element, in pairs. The loop issues about 100 instructions for a block's 16
 // exponentials a lane, so that the exponentials (a quarter of a warp's lanes a
 // cycle) and not the issue come next after the memory.
 //
@@ -76,6 +76,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=l"(reinterpret_cast<uint64_t&>(d))
       : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
         "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -214,14 +221,18 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
 }
 
 // A lane's running sums, all lanes of a warp with the same m. S is kept over
-// log2(e), and so is the exponent's m: t = x log2(e) - m2.
+// ln(2): its terms are e^(x - m) t with the exponent t = (x - m) log2(e). The maximum is
+// subtracted before the scaling. fma(x, log2(e), -m log2(e)) would save one of five
+// packed instructions (4096 rows of bf16 in a loop: 251 us, 254.5 so), but its exponents are
+// all off by the rounding of m log2(e): by 1e-3 at |m| = 3e4, differently for each m that
+// the running maximum took on, and by hundreds at |m| = 1e10.
 template <typename T>
 struct Running {
   // Below (or, bf16 and fp32, above) these, two values of T that differ do so by
   // 32 at least: the maximum's equals have the weight 1 and the others 1e-14 at most.
   static constexpr float kFarLow = std::is_same<T, __half>::value ? -60000.f : -0.9e30f;
   static constexpr float kFarHigh = 0.9e30f;
-  float m = -INFINITY, m2 = -INFINITY;
+  float m = -INFINITY;
   float2 z = {0.f, 0.f}, s = {0.f, 0.f};
 
   // A block whose largest element over the warp is `most`.
@@ -233,14 +244,13 @@ struct Running {
       s = make_float2((s.x + z.x * d) * c, (s.y + z.y * d) * c);
       z = make_float2(z.x * c, z.y * c);
       m = most;
-      m2 = m * kLog2e;
     }
     if (m > kFarLow && m < kFarHigh) {
       b.lift();
-      const float2 l2 = make_float2(kLog2e, kLog2e), nm = make_float2(-m2, -m2);
+      const float2 l2 = make_float2(kLog2e, kLog2e), nm = make_float2(-m, -m);
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
-        const float2 t = fma2(b.pair(p), l2, nm);
+        const float2 t = mul2(add2(b.pair(p), nm), l2);
         const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
         z = add2(z, e);
         s = fma2(e, t, s);
@@ -254,19 +264,13 @@ struct Running {
       }
     }
   }
-  // Over the warp. The exponents had the rounded m2 where m log2(e) is meant;
-  // both sums are put right for the difference.
+  // Over the warp.
   __device__ __forceinline__ Sums all() const {
     Sums r = {m, z.x + z.y, s.x + s.y};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       r.z += __shfl_xor_sync(0xffffffffu, r.z, o);
       r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
-    }
-    if (m > kFarLow && m < kFarHigh) {
-      const float off = fmaf(-m, kLog2e, m2), c = exp2f(off);
-      r.s = (r.s + r.z * off) * c;
-      r.z *= c;
     }
     r.s *= kLn2;
     return r;

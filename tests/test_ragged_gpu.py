@@ -526,6 +526,38 @@ def test_token_logprobs_hard_rows(dtype):
     _check_logprobs(x, torch.full((x.shape[0],), 4321, device=DEV), k)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("repeat", [1, 25])
+def test_token_logprobs_finite_fills(dtype, repeat):
+    """Rows, and blocks of rows, filled with a finite value of large magnitude, as
+    masks do; few rows (split over CTAs) and many (a CTA each)."""
+    V, k = 5001, 20
+    g = _gen(11)
+    base = _randn(g, V, dtype=dtype, scale=3.0)
+    rows = []
+    for c in (-1e9, -1e10, -1e12, -1e20, -1e29, 1e9, 1e10, 1e20, 1e29):
+        first, last, one = base.clone(), base.clone(), base.clone()
+        first[:1024] = c
+        last[:4608] = c
+        one[2048:2560] = c
+        steps = torch.full_like(base, c) * (1 + torch.randint(3, (V,), generator=g, device=DEV)
+                                            * 2.0 ** (-7 if dtype == torch.bfloat16 else -23))
+        rows += [torch.full_like(base, c), first, last, one, steps.to(dtype)]
+    x = torch.stack(rows).repeat(repeat, 1)
+    _check_logprobs(x, torch.randint(V, (x.shape[0],), generator=g, device=DEV), k)
+
+
+@pytest.mark.parametrize("shift", [0.0, 1e3, 1e4, 3e4, 1e6, -1e6, 3e7])
+def test_token_logprobs_shifted_rows_that_rise(shift):
+    """A maximum that moves from block to block of a warp, far from zero: the sums
+    so far keep their weight."""
+    g = _gen(12)
+    x = (torch.randn(600, 20000, generator=g, device=DEV) * 3.0).sort(dim=-1).values
+    x[300:] = x[300:, torch.randperm(20000, generator=g, device=DEV)]
+    x += shift
+    _check_logprobs(x, torch.randint(20000, (600,), generator=g, device=DEV), 5)
+
+
 def test_token_logprobs_no_distribution():
     V = 3000
     x = torch.randn(5, V, device=DEV)
