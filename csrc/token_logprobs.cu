@@ -248,13 +248,18 @@ struct Running {
     if (m > kFarLow && m < kFarHigh) {
       b.lift();
       const float2 l2 = make_float2(kLog2e, kLog2e), nm = make_float2(-m, -m);
+      // The block by itself first: a long row's sums then meet 8 times fewer
+      // roundings, which for equal logits all go the same way.
+      float2 zb, sb;
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
         const float2 t = mul2(add2(b.pair(p), nm), l2);
         const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-        z = add2(z, e);
-        s = fma2(e, t, s);
+        zb = p == 0 ? e : add2(zb, e);
+        sb = p == 0 ? mul2(e, t) : fma2(e, t, sb);
       }
+      z = add2(z, zb);
+      s = add2(s, sb);
     } else if (m > -INFINITY) {
 #pragma unroll
       for (int p = 0; p < 8; ++p) {

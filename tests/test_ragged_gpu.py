@@ -493,6 +493,23 @@ def _check_logprobs(x, ids, k):
     assert r.top_ids.shape == r.top_logprobs.shape == (x.shape[0], k)
 
 
+def _near_logprobs(r, x, ids, k):
+    """``_check_logprobs`` of a result that is there."""
+    xd = x.double()
+    ls = xd - xd.amax(-1, keepdim=True)
+    ls = ls - ls.exp().sum(-1, keepdim=True).log()
+    p = ls.exp()
+    ent = -torch.where(p == 0, torch.zeros_like(p), p * ls).sum(-1)
+    top = torch.sort(xd + 0.0, dim=-1, descending=True, stable=True).indices[:, :k]
+    for got, want in ((r.logprob, ls.gather(1, ids[:, None])[:, 0]), (r.entropy, ent),
+                      (r.top_logprobs, ls.gather(1, top))):
+        off = (got.double() - want).abs()
+        off = torch.where(got.double() == want, torch.zeros_like(off), off)
+        worst = (off / want.abs().clamp_min(1.0)).nan_to_num(math.inf, math.inf)
+        assert bool((worst <= 2.0 ** -20).all()), float(worst.max())
+    assert torch.equal(r.top_ids, top)
+
+
 @pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 2, 2), (2, 31, 5), (5, 255, 32), (4, 256, 0),
                                    (7, 257, 20), (1, 50257, 20), (33, 4096, 8), (2, 151936, 32),
                                    (300, 1000, 3), (1, 300000, 20), (0, 100, 5)])
@@ -545,6 +562,33 @@ def test_token_logprobs_finite_fills(dtype, repeat):
         rows += [torch.full_like(base, c), first, last, one, steps.to(dtype)]
     x = torch.stack(rows).repeat(repeat, 1)
     _check_logprobs(x, torch.randint(V, (x.shape[0],), generator=g, device=DEV), k)
+
+
+def _many_blocks(g, R, V, dtype):
+    """Rows of V logits that rise, fall, are shifted and have their first blocks
+    masked, in turn."""
+    x = _randn(g, R, V, dtype=dtype, scale=3.0)
+    x[0::6] = x[0::6].sort(dim=-1).values
+    x[1::6] = x[1::6].sort(dim=-1, descending=True).values
+    x[2::6, : V - 100] = -math.inf
+    x[3::6, : V // 2] = -1e4
+    x[4::6] = (x[4::6].float() - 30000.0).to(dtype)
+    return x
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("R,V,k,offset", [(600, 50257, 20, 7), (1200, 50264, 3, 0),
+                                          (700, 20000, 32, 0), (600, 262656, 5, 0)])
+def test_token_logprobs_many_blocks_a_warp(R, V, k, offset, dtype):
+    """One CTA a row, several blocks a warp: rows on the 16-byte grid and off it."""
+    g = _gen(R)
+    x = torch.zeros(R, V + offset, dtype=dtype, device=DEV)[:, offset:]
+    x.copy_(_many_blocks(g, R, V, dtype))
+    ids = torch.randint(V, (R,), generator=g, device=DEV)
+    for a in range(0, R, 200):  # the 64-bit form in pieces, the operator on all rows
+        r = ops.token_logprobs(x, ids, k)
+        _near_logprobs(ops.TokenLogprobs(*(t[a:a + 200] for t in r)), x[a:a + 200],
+                       ids[a:a + 200], k)
 
 
 @pytest.mark.parametrize("shift", [0.0, 1e3, 1e4, 3e4, 1e6, -1e6, 3e7])
