@@ -466,7 +466,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         float p[4], r[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[e] = m[n][e & 1] == -INFINITY ? 0.f : exp2_approx(x[e] - m[n][e & 1]);
+          // a masked key weighs nothing; a score that is NaN, which no maximum holds, stays
+          p[e] = x[e] == -INFINITY ? 0.f : exp2_approx(x[e] - m[n][e & 1]);
           r[e] = p[e] - to_f(from_f<T>(p[e]));
         }
         l[n][0] += p[0] + p[2];
@@ -530,7 +531,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float2 s = ml[w * 8 + h];
-          const float c = s.x == -INFINITY ? 0.f : exp2_approx(s.x - M);
+          // by the sum: of a warp whose scores are all NaN the maximum is -inf too
+          const float c = s.y == 0.f ? 0.f : exp2_approx(s.x - M);
           const float4 v = *reinterpret_cast<const float4*>(join + join_at<D>(w, h, d));
           lsum += s.y * c;
           acc.x += v.x * c;
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const uint8_t* at = smem + p * P::kBytes;
             const float2 s = reinterpret_cast<const float2*>(at)[hd];
             const float4 v = *reinterpret_cast<const float4*>(at + P::kStats + (hd * D + d) * 4);
-            const float f = s.x == -INFINITY ? 0.f : exp2_approx(s.x - m_new);
+            const float f = s.y == 0.f ? 0.f : exp2_approx(s.x - m_new);
             lsum[t] += s.y * f;
             acc[t].x += v.x * f;
             acc[t].y += v.y * f;

@@ -143,6 +143,37 @@ def test_paged_decode_large_scores_and_scale():
         _close(out[b:b + 1], _exact_rows(q[b:b + 1], *dense[b], scale=0.003), torch.bfloat16)
 
 
+@pytest.mark.parametrize("nq,nkv,D", [(8, 2, 128), (32, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("lens", [[1, 40, 300, 16], [9000], [20, 30000, 1]])
+def test_paged_decode_nan_is_kept(nq, nkv, D, lens):
+    """NaN in a query, in one key, in a block of keys and in every key reach the
+    heads that see them and no others: items of one CTA and items cut over several."""
+    g = _gen(13)
+    G, page = nq // nkv, 32
+    kp, vp, table, dense = _pool(g, lens, nkv, D, page, torch.bfloat16)
+    q = _randn(g, len(lens), nq, D)
+    seq = _i32(lens)
+    want = ops.paged_decode_attention(q, kp, vp, table, seq).view(len(lens), nq, D)
+    assert want.isfinite().all()
+
+    def check(got, b, heads):
+        got = got.view(len(lens), nq, D)
+        hit = torch.zeros(len(lens), nq, dtype=torch.bool, device=DEV)
+        hit[b, heads] = True
+        assert got[hit].isnan().all() and torch.equal(got[~hit], want[~hit])
+
+    b = lens.index(max(lens))
+    q2 = q.clone()
+    q2[b, nq - 2, 5] = NAN
+    check(ops.paged_decode_attention(q2, kp, vp, table, seq), b, [nq - 2])
+    for b, n in enumerate(lens):
+        for first, count in ((0, 1), (n - 1, 1), (n // 2 // 16 * 16, 16), (0, n)):
+            k2 = kp.clone()
+            at = torch.arange(first, min(n, first + count), device=DEV)
+            k2[table[b].long()[at // page], 1, at % page, 3] = NAN
+            check(ops.paged_decode_attention(q, k2, vp, table, seq), b, list(range(G, 2 * G)))
+
+
 def test_paged_decode_strides():
     """q as a view of a projection; the pool as a layer of a larger buffer, with
     k and v interleaved page by page; a table wider than its view."""
