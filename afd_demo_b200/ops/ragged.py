@@ -94,10 +94,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal GQA attention of packed sequences: q [T, nq, D], k and v
     [Tk, n_kv, D] (any row stride, e.g. views of one projection), sequence i in
-    rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32 [n + 1], from 0 up). With
+    rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32 [n + 1], rising). With
     `cu_seqlens_k` the keys have rows of their own and the queries are the last
     positions of their sequence; a query before the first key gives zeros, and so
-    do rows past cu_seqlens[n]. Returns [T, nq * D]."""
+    do rows before cu_seqlens[0] and past cu_seqlens[n]. Returns [T, nq * D]."""
     if not q.is_cuda:
         return torch_ref.packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale)
     return _ext().packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale, status)

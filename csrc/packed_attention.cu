@@ -202,6 +202,20 @@ struct Smem {
       2 * kQTile + 2 * kStages * kKvTile + 8 * kStage + 1024 /*align*/ + 512;
 };
 
+// Zeros for the rows that no sequence owns and no item stores, those before the
+// first offset: each CTA's share of them, by the softmax warps while the first item's
+// queries and keys are on their way. A call, so that the loop behind it keeps its
+// registers (inlined, it spilled 48 bytes).
+__device__ __noinline__ void zero_unowned(const int* cu_q, int T, int nq, int D, void* out,
+                                          int* n_parts) {
+  const size_t rows = (size_t)min(max(cu_q[0], 0), T) * nq;
+  const size_t first = (size_t)blockIdx.x * 256 + threadIdx.x - 64, step = (size_t)gridDim.x * 256;
+  for (size_t i = first; i < rows * (D / 8); i += step)
+    reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+  if (n_parts != nullptr)
+    for (size_t i = first; i < rows; i += step) n_parts[i] = 1;
+}
+
 }  // namespace
 
 template <typename T, int D, bool kPaged>
@@ -300,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int q0 = cu_q(lo), q1 = lo < a.n_seqs ? max(cu_q(lo + 1), q0) : a.T;
       const int blocks = (q1 - q0 + block_tokens - 1) / block_tokens;
       int block = blocks - 1 - (slot - (q0 / block_tokens + lo));
+      if (block >= blocks) block = -1;  // a slot before the first sequence's
       int k0 = 0, len = 0;
       if (lo < a.n_seqs && block >= 0) {
         if (lane == 0 && (a.cu_q[lo] != q0 || a.cu_q[lo + 1] != q1))
@@ -510,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------- softmax, O, output rows
+    zero_unowned(a.cu_q, a.T, a.nq, D, a.out, a.splits > 1 ? a.n_parts : nullptr);
     const int x = (warp - 2) / 4;         // row tile of this warp group
     const int qq = warp & 3;              // TMEM lane quarter of this warp
     const int row = qq * 32 + lane;

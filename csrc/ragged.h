@@ -49,8 +49,8 @@ int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s);
 // cu_q[i] .. cu_q[i+1] - 1; they are its last positions. Keys and values come
 // packed (k, v, cu_k: key rows of the sequences) or from pages (seq_lens: all
 // positions, the new ones included). A query whose position is negative
-// (more queries than keys) sees no key and gets zeros, and so do rows past
-// cu_q[n]. Offsets outside [0, rows] or decreasing are clamped and recorded;
+// (more queries than keys) sees no key and gets zeros, and so do rows before
+// cu_q[0] and past cu_q[n]. Offsets outside [0, rows] or decreasing are clamped and recorded;
 // lengths and page ids as in PagedDecodeArgs.
 struct PackedAttnArgs {
   const void* q;            // [T, nq, D], rows q_row elements apart

@@ -327,6 +327,41 @@ def test_packed_attention_neighbours_do_not_mix():
         assert torch.equal(out[:100], want[:100]) and torch.equal(out[160:], want[160:])
 
 
+def _leave_nan(rows, width):
+    """NaN where the next output of this size will lie."""
+    torch.full((rows, width), NAN, device=DEV, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("first", [1, 31, 32, 37, 300])
+@pytest.mark.parametrize("nq,nkv,D", [(32, 4, 128), (4, 2, 64)])
+def test_packed_attention_rows_before_the_first_offset(first, nq, nkv, D):
+    """They get zeros, as the rows past the last offset do, and the sequences what
+    they get without them; also where the keys are split."""
+    g = _gen(14)
+    lens, after = [60, 0, 200, 3], 41
+    T = first + sum(lens) + after
+    q = _randn(g, T, nq, D, scale=2.0)
+    k, v = _randn(g, T, nkv, D), _randn(g, T, nkv, D)
+    cu = _cu(lens) + first
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    _leave_nan(T, nq * D)
+    out = ops.packed_attention(q, k, v, cu, status=status)
+    a = first
+    for n in lens:
+        _close(out[a:a + n], _exact_rows(q[a:a + n], k[a:a + n], v[a:a + n]), torch.bfloat16)
+        a += n
+    assert not out[:first].any() and not out[a:].any()
+    totals = [5000, 40]
+    kp, vp, table, dense = _pool(g, totals, nkv, D, 64, torch.bfloat16)
+    T = first + 8 + 5
+    _leave_nan(T, nq * D)
+    out = ops.paged_prefill_attention(q[:T], kp, vp, table, _i32(totals),
+                                      _i32([first, first + 8, T]), status=status)
+    _close(out[first:first + 8], _exact_rows(q[first:first + 8], *dense[0]), torch.bfloat16)
+    _close(out[first + 8:], _exact_rows(q[first + 8:T], *dense[1]), torch.bfloat16)
+    assert not out[:first].any() and status.tolist()[0] == 0
+
+
 def test_packed_attention_bad_offsets_are_recorded():
     g = _gen(9)
     q, k, v = (_randn(g, 64, 2, 64) for _ in range(3))
