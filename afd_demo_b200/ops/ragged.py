@@ -13,7 +13,8 @@ graphs; the lengths, tables and offsets are read on the device at each replay.
 On CPU tensors they run the PyTorch statements of ``torch_ref``. Wrong types,
 shapes or devices raise ValueError. Index data is checked on the device: an
 entry out of range is never dereferenced and is recorded in the optional
-``status`` word pair (int32 [2], code 3), as the other kernels do.
+``status`` word pair (int32 [2], code 3), as the other kernels do. Offsets of rows
+are clamped to the rows there are; query offsets that decrease give zeros throughout.
 """
 
 from __future__ import annotations

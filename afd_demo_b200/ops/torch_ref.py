@@ -281,6 +281,14 @@ def _paged_rows(pages: torch.Tensor, table: torch.Tensor, n: int) -> torch.Tenso
     return x.transpose(1, 2).reshape(-1, pages.shape[1], pages.shape[3])[:n]
 
 
+def _offsets(cu: torch.Tensor, rows: int) -> List[int]:
+    return [min(max(c, 0), rows) for c in cu.tolist()]
+
+
+def _decrease(offsets: List[int]) -> bool:
+    return any(b < a for a, b in zip(offsets, offsets[1:]))
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None
                      ) -> torch.Tensor:
@@ -294,7 +302,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         _check(c.dtype == torch.int32 and c.numel() == cu_seqlens.numel() >= 1,
                "cu_seqlens must hold n + 1 int32 offsets")
     out = torch.zeros(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
-    cq, ck = cu_seqlens.tolist(), cu_k.tolist()
+    cq, ck = _offsets(cu_seqlens, q.shape[0]), _offsets(cu_k, k.shape[0])
+    if _decrease(cq):
+        return out
     for i in range(len(cq) - 1):
         if cq[i + 1] > cq[i] and ck[i + 1] > ck[i]:
             out[cq[i]:cq[i + 1]] = _causal_rows(q[cq[i]:cq[i + 1]], k[ck[i]:ck[i + 1]],
@@ -315,7 +325,9 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     _check(page_table.dim() == 2 and page_table.shape[0] == n and seq_lens.numel() == n,
            f"page_table and seq_lens must have a row for each of the {n} sequences")
     out = torch.zeros(q.shape[0], q.shape[1] * q.shape[2], dtype=q.dtype, device=q.device)
-    cq = cu_seqlens.tolist()
+    cq = _offsets(cu_seqlens, q.shape[0])
+    if _decrease(cq):
+        return out
     for i in range(n):
         m = int(seq_lens[i])
         if cq[i + 1] > cq[i] and m > 0:

@@ -202,18 +202,39 @@ struct Smem {
       2 * kQTile + 2 * kStages * kKvTile + 8 * kStage + 1024 /*align*/ + 512;
 };
 
-// Zeros for the rows that no sequence owns and no item stores, those before the
-// first offset: each CTA's share of them, by the softmax warps while the first item's
-// queries and keys are on their way. A call, so that the loop behind it keeps its
-// registers (inlined, it spilled 48 bytes).
-__device__ __noinline__ void zero_unowned(const int* cu_q, int T, int nq, int D, void* out,
-                                          int* n_parts) {
-  const size_t rows = (size_t)min(max(cu_q[0], 0), T) * nq;
-  const size_t first = (size_t)blockIdx.x * 256 + threadIdx.x - 64, step = (size_t)gridDim.x * 256;
+// What the softmax warps (256 threads) do while the first item's queries and keys
+// are on their way: check the query offsets, and store zeros, each CTA its share, to the
+// rows that no item stores: those before the first offset, or all rows where offsets
+// decrease. Such a list gives some rows two owners and others none, so then (true)
+// no item stores anything. Every CTA reads the whole list and comes to the same
+// answer: n / 256 loads a thread, against n * nkv / 148 items of a microsecond or more.
+// A call, so that the loop behind it keeps its registers (inlined, it spilled 48 bytes).
+__device__ __noinline__ bool settle_offsets(const int* cu_q, int n, int T, int nq, int D, void* out,
+                                            int* n_parts, int* status) {
+  const int id = threadIdx.x - 64;
+  bool outside = false, down = false;
+  for (int i = id; i <= n; i += 256) {
+    const int c = cu_q[i], next = cu_q[min(i + 1, n)];
+    outside |= c < 0 || c > T;
+    down |= min(max(next, 0), T) < min(max(c, 0), T);
+  }
+  if ((outside || down) && blockIdx.x == 0) report_status(status, kBoundsViolation, 210);
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, 1, 256, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)down)
+      : "memory");
+  const size_t rows = (size_t)(any ? T : min(max(cu_q[0], 0), T)) * nq;
+  const size_t first = (size_t)blockIdx.x * 256 + id, step = (size_t)gridDim.x * 256;
   for (size_t i = first; i < rows * (D / 8); i += step)
     reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
   if (n_parts != nullptr)
     for (size_t i = first; i < rows; i += step) n_parts[i] = 1;
+  return any;
 }
 
 }  // namespace
@@ -317,8 +338,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (block >= blocks) block = -1;  // a slot before the first sequence's
       int k0 = 0, len = 0;
       if (lo < a.n_seqs && block >= 0) {
-        if (lane == 0 && (a.cu_q[lo] != q0 || a.cu_q[lo + 1] != q1))
-          report_status(a.status, kBoundsViolation, 210);
         if (kPaged) {
           len = checked_len(a.seq_lens[lo], a.max_pages * a.page_size, a.status, 211);
         } else {
@@ -525,12 +544,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------- softmax, O, output rows
-    zero_unowned(a.cu_q, a.T, a.nq, D, a.out, a.splits > 1 ? a.n_parts : nullptr);
+    const int stored_rows =  // of a tile
+        settle_offsets(a.cu_q, a.n_seqs, a.T, a.nq, D, a.out, a.splits > 1 ? a.n_parts : nullptr,
+                       a.status)
+            ? 0
+            : tok1 * G;
     const int x = (warp - 2) / 4;         // row tile of this warp group
     const int qq = warp & 3;              // TMEM lane quarter of this warp
     const int row = qq * 32 + lane;
     const int tok = x * tok1 + row / G;   // this row's token in the block
-    const bool has_token = row < tok1 * G;
+    const bool has_token = row < stored_rows;
     const int tok_first = x * tok1 + (qq * 32) / G;  // of the warp's first row
     const uint32_t lane_off = (uint32_t)(qq * 32) << 16;
     const uint32_t t_o = tmem + 256 + x * 128 + lane_off;
@@ -689,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int rw = k * 4 + lane / 8, r = qq * 32 + rw, t = r / G;
-            if (r < tok1 * G && x * tok1 + t < w.tokens)
+            if (r < stored_rows && x * tok1 + t < w.tokens)
               *reinterpret_cast<uint4*>(out + ((size_t)t * a.nq + (r - t * G)) * D + c * kDims) =
                   *reinterpret_cast<const uint4*>(stage + rw * 128 +
                                                   ((lane % 8 ^ (rw & 7)) << 4));

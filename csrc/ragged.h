@@ -50,8 +50,10 @@ int launch_paged_decode(const PagedDecodeArgs& a, int num_sms, cudaStream_t s);
 // packed (k, v, cu_k: key rows of the sequences) or from pages (seq_lens: all
 // positions, the new ones included). A query whose position is negative
 // (more queries than keys) sees no key and gets zeros, and so do rows before
-// cu_q[0] and past cu_q[n]. Offsets outside [0, rows] or decreasing are clamped and recorded;
-// lengths and page ids as in PagedDecodeArgs.
+// cu_q[0] and past cu_q[n]. Offsets outside [0, rows] are clamped and recorded; with
+// query offsets that still decrease then, which is recorded too, all rows get zeros,
+// and with key offsets that do, the sequence has no key. Lengths and page ids as in
+// PagedDecodeArgs. A call without rows of queries, or of keys, checks no offset.
 struct PackedAttnArgs {
   const void* q;            // [T, nq, D], rows q_row elements apart
   long long q_row;

@@ -138,3 +138,22 @@ def test_refusals():
                 (x, torch.zeros(2).long(), 10), (x.double(), torch.zeros(2).long(), 1)):
         with pytest.raises(ValueError):
             ops.token_logprobs(*bad)
+
+
+@pytest.mark.parametrize("cu,same", [([0, 10, 5, 12], None), ([9, 0], None),
+                                     ([0, 8, 70], [0, 8, 12]), ([-3, 5, 12], [0, 5, 12]),
+                                     ([4, 6, 9], [4, 6, 9])])
+def test_query_offsets_are_clamped_and_decreasing_ones_give_zeros(cu, same):
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(12, h, 32, generator=g) for h in (4, 2, 2))
+    n = len(cu) - 1
+    kp, vp, table, _ = _pool([20] * n, 2, 32, 16, g)
+    for call in (lambda c: ops.packed_attention(q, k, v, _i32(c)),
+                 lambda c: ops.paged_prefill_attention(q, kp, vp, table, _i32([20] * n), _i32(c))):
+        out = call(cu)
+        if same is None:
+            assert not out.any()
+        else:
+            assert torch.equal(out, call(same))
+            assert not out[: same[0]].any() and not out[same[-1]:].any()
+            assert out[same[0]: same[-1]].any(-1).all()

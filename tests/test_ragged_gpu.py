@@ -372,6 +372,32 @@ def test_packed_attention_bad_offsets_are_recorded():
     assert status.tolist()[0] == 3
 
 
+@pytest.mark.parametrize("cu,T", [([0, 10, 5, 12], 12), ([0, 200, 40, 300], 300), ([9, 0], 40),
+                                  ([0, 64, 70], 64), ([-3, 20, 64], 64), ([0, 1 << 30, 64], 64),
+                                  (list(range(700)) + [698, 700], 700)])
+def test_packed_attention_bad_query_offsets(cu, T):
+    """Recorded, and a defined output: what the clamped offsets give, or zeros where
+    they decrease; whole keys and split ones; the next call is not disturbed."""
+    g = _gen(15)
+    q, k, v = _randn(g, T, 8, 128), _randn(g, T, 2, 128), _randn(g, T, 2, 128)
+    n = len(cu) - 1
+    kp, vp, table, _ = _pool(g, [3000 if n < 10 else 20] * n, 2, 128, 64, torch.bfloat16)
+    lens = _i32([3000 if n < 10 else 20] * n)
+    clamped = [min(max(c, 0), T) for c in cu]
+    for call in (lambda c, s=None: ops.packed_attention(q, k, v, _i32(c), status=s),
+                 lambda c, s=None: ops.paged_prefill_attention(q, kp, vp, table, lens, _i32(c),
+                                                               status=s)):
+        good = [0] * n + [T]
+        before = call(good)
+        want = call(clamped) if clamped == sorted(clamped) else torch.zeros_like(before)
+        for _ in range(2):
+            status = torch.zeros(2, dtype=torch.int32, device=DEV)
+            _leave_nan(T, 8 * 128)
+            out = call(cu, status)
+            assert status.tolist()[0] == 3 and torch.equal(out, want)
+        assert torch.equal(call(good), before)
+
+
 @pytest.mark.parametrize("nq,nkv,D", [(32, 4, 128), (16, 2, 64), (6, 2, 128)])
 @pytest.mark.parametrize("page", [16, 48, 64, 128, 256])
 def test_paged_prefill(nq, nkv, D, page):
