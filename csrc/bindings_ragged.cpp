@@ -87,14 +87,22 @@ at::Tensor loadable(const at::Tensor& t, bool ok) {
   return ok || t.numel() == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-// [rows, heads, D] with contiguous heads and 16-byte aligned rows.
+// [rows, heads, D] with contiguous heads and 16-byte aligned rows that do not
+// overlap: a tensor map gets their distance, so rows expanded from one are copied.
 at::Tensor take_rows(const at::Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(t.is_cuda(), what, " must be a CUDA tensor");
   TORCH_CHECK_VALUE(t.dim() == 3, what, " must be [rows, heads, head_dim]");
   TORCH_CHECK_VALUE(t.size(2) == 64 || t.size(2) == 128, what, ": head_dim must be 64 or 128");
   TORCH_CHECK_VALUE(t.size(0) < (1ll << 31), what, ": too many rows");
   return loadable(t, t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == t.size(2)) &&
-                         t.stride(0) % 8 == 0 && t.stride(0) >= 0 && aligned16(t.data_ptr()));
+                         (t.size(0) == 1 ||
+                          (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2))) &&
+                         aligned16(t.data_ptr()));
+}
+
+// Elements between the rows of what take_rows gave; a single row has any stride.
+int64_t row_of(const at::Tensor& t) {
+  return t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0);
 }
 
 void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* what) {
@@ -181,7 +189,7 @@ at::Tensor paged_decode_attention(const at::Tensor& q_in, const at::Tensor& k_pa
   check_ints(seq_lens, q, a.B, "seq_lens");
   at::Tensor out = at::empty({a.B, (int64_t)a.nq * a.D}, q.options());
   a.q = q.data_ptr();
-  a.q_row = q.stride(0);
+  a.q_row = row_of(q);
   a.k_pages = k_pages.data_ptr();
   a.v_pages = v_pages.data_ptr();
   a.seq_lens = seq_lens.data_ptr<int>();
@@ -214,7 +222,7 @@ at::Tensor packed_common(PackedAttnArgs& a, const at::Tensor& q, const at::Tenso
   a.n_seqs = (int)cu_q.numel() - 1;
   at::Tensor out = at::empty({a.T, (int64_t)a.nq * a.D}, q.options());
   a.q = q.data_ptr();
-  a.q_row = q.stride(0);
+  a.q_row = row_of(q);
   a.cu_q = cu_q.data_ptr<int>();
   a.out = out.data_ptr();
   a.scale = scale_of(scale, a.D);
@@ -252,8 +260,8 @@ at::Tensor packed_attention(const at::Tensor& q_in, const at::Tensor& k_in, cons
   check_ints(cu_k, q, cu_q.numel(), "cu_seqlens_k");
   a.k = k.data_ptr();
   a.v = v.data_ptr();
-  a.k_row = k.stride(0);
-  a.v_row = v.stride(0);
+  a.k_row = row_of(k);
+  a.v_row = row_of(v);
   a.Tk = (int)k.size(0);
   a.cu_k = cu_k.data_ptr<int>();
   run_packed(a, q, a.Tk, "packed_attention");

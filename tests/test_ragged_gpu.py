@@ -362,6 +362,31 @@ def test_packed_attention_rows_before_the_first_offset(first, nq, nkv, D):
     assert not out[:first].any() and status.tolist()[0] == 0
 
 
+@pytest.mark.parametrize("T", [1, 200])
+def test_attention_of_rows_that_share_memory(T):
+    """One row expanded to many, rows that overlap, and single rows of any stride."""
+    g = _gen(16)
+    flat = _randn(g, T * 8 + 4 * 64)
+
+    def forms(h):
+        yield _randn(g, 1, h, 64).expand(T, h, 64)
+        yield flat.as_strided((T, h, 64), (8, 64, 1))
+        if T == 1:
+            yield flat.as_strided((1, h, 64), (3, 64, 1))
+
+    cu, dec = _cu([T]), torch.zeros(T, 1, dtype=torch.int32, device=DEV)
+    kp, vp = _randn(g, 1, 2, 64, 64), _randn(g, 1, 2, 64, 64)
+    for q in forms(4):
+        for k in forms(2):
+            v = next(forms(2))
+            out = ops.packed_attention(q, k, v, cu)
+            assert torch.equal(out, ops.packed_attention(*(x.contiguous() for x in (q, k, v)), cu))
+            _close(out, _exact_rows(q, k, v), torch.bfloat16)
+        args = (kp, vp, dec, torch.full((T,), 40, dtype=torch.int32, device=DEV))
+        assert torch.equal(ops.paged_decode_attention(q, *args),
+                           ops.paged_decode_attention(q.contiguous(), *args))
+
+
 def test_packed_attention_bad_offsets_are_recorded():
     g = _gen(9)
     q, k, v = (_randn(g, 64, 2, 64) for _ in range(3))
