@@ -25,6 +25,7 @@ import torch
 
 from .. import ops
 from ..config import ModelConfig
+from ..ops.checks import AFDBoundsError
 from ..utils.sampling import sample_next_token
 from .attention import AttentionWorker
 from .ffn import FFNWorker
@@ -106,7 +107,9 @@ def slots_of(table: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor,
 
 class RaggedGenerator:
     """Serves batches of prompts of different lengths on the workers of one
-    process. `num_pages` * `page_size` positions are held at once."""
+    process. `num_pages` * `page_size` positions are held at once. Every call reads
+    once, at its end, what its kernels recorded: AFDBoundsError for an index out of
+    range, RuntimeError for a wait inside a kernel that ran out."""
 
     def __init__(self, attention: AttentionWorker, ffn: FFNWorker, num_pages: int,
                  page_size: int = 64):
@@ -117,6 +120,8 @@ class RaggedGenerator:
         self.max_positions = attention.rope.shape[0]
         self.cache = PagedKVCache(attention.cfg, num_pages, page_size, attention.device,
                                   attention.dtype)
+        cuda = attention.device.type == "cuda"
+        self.status = torch.zeros(2, dtype=torch.int32, device=self.device) if cuda else None
 
     # ------------------------------------------------------------- helpers
     def _check_prompts(self, prompts: Sequence[Sequence[int]], new: int) -> List[torch.Tensor]:
@@ -135,6 +140,16 @@ class RaggedGenerator:
             got.append(t)
         return got
 
+    def _check_status(self) -> None:
+        """Raises what the kernels since the last check recorded (waits for them)."""
+        if self.status is None:
+            return
+        code, site = self.status.tolist()
+        if code != 0:
+            self.status.zero_()
+            error = AFDBoundsError if code == 3 else RuntimeError
+            raise error(f"a kernel recorded a failure: code={code} site={site}")
+
     def _forward(self, ids: torch.Tensor, attend) -> torch.Tensor:
         """Every layer on the packed tokens `ids` [T]; attend(layer, qkv, lw) ->
         [T, nq * D]. Returns the hidden states [T, H]."""
@@ -152,7 +167,7 @@ class RaggedGenerator:
         kp, vp = self.cache.layer(l)
         return ops.qk_norm_rope_paged(qkv, lw.q_norm, lw.k_norm, self.aw.rope, kp, vp, positions,
                                       slots, cfg.num_attention_heads, cfg.num_key_value_heads,
-                                      cfg.rms_norm_eps)
+                                      cfg.rms_norm_eps, status=self.status)
 
     def _prefill(self, prompts: List[torch.Tensor], table: torch.Tensor,
                  chunk: Optional[int]) -> torch.Tensor:
@@ -177,7 +192,7 @@ class RaggedGenerator:
             def attend(l, qkv, lw):
                 q = self._store(l, qkv, lw, pos, slots)
                 kp, vp = self.cache.layer(l)
-                return ops.paged_prefill_attention(q, kp, vp, tab, total, cu)
+                return ops.paged_prefill_attention(q, kp, vp, tab, total, cu, status=self.status)
 
             x = self._forward(ids, attend)
             for j, i in enumerate(live):
@@ -230,10 +245,11 @@ class RaggedGenerator:
                 def attend(l, qkv, lw):
                     q = self._store(l, qkv, lw, pos, slots)
                     kp, vp = self.cache.layer(l)
-                    return ops.paged_decode_attention(q, kp, vp, table, lens)
+                    return ops.paged_decode_attention(q, kp, vp, table, lens, status=self.status)
 
                 logits = self._logits(self._forward(tok, attend))
                 pos = lens
+            self._check_status()
         finally:
             for s in seqs:
                 self.cache.release(s)
@@ -266,14 +282,15 @@ class RaggedGenerator:
         def attend(l, qkv, lw):
             q, k, v = ops.qk_norm_rope_packed(qkv, lw.q_norm, lw.k_norm, self.aw.rope, pos,
                                               cfg.num_attention_heads, cfg.num_key_value_heads,
-                                              cfg.rms_norm_eps)
-            return ops.packed_attention(q, k, v, cu)
+                                              cfg.rms_norm_eps, status=self.status)
+            return ops.packed_attention(q, k, v, cu, status=self.status)
 
         x = self._forward(flat, attend)
         after = torch.cat([torch.cat([p[1:], p[:1] * 0]) for p in ids]).to(dev)
         parts = [ops.token_logprobs(self._logits(x[a:a + rows_at_once]),
                                     after[a:a + rows_at_once], top_logprobs)
                  for a in range(0, x.shape[0], rows_at_once)]
+        self._check_status()
         whole = [torch.cat([p[f] for p in parts]) for f in range(4)]
         out, a = [], 0
         for n in lens:  # a sequence's last row has no token after it

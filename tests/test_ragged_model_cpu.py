@@ -100,3 +100,17 @@ def test_paged_cache_reuses_pages():
     d = c.allocate(80)
     assert c.free_pages == 0 and held <= set(c.table([d])[0].tolist())
     assert not set(c.table([b])[0, :1].tolist()) & set(c.table([d])[0].tolist())
+
+
+@pytest.mark.parametrize("code", [1, 3])
+def test_what_a_kernel_recorded_is_raised_once(model, code):
+    from afd_demo_b200.ops.checks import AFDBoundsError
+
+    gen = model.ragged(num_pages=2, page_size=16)
+    p = _prompts(model, [5])
+    for call in (lambda: gen.generate(p, 2), lambda: gen.score(p)):
+        gen.status = torch.tensor([code, 223], dtype=torch.int32)
+        with pytest.raises(AFDBoundsError if code == 3 else RuntimeError, match="site=223"):
+            call()
+        assert gen.cache.free_pages == 2
+        call()

@@ -63,3 +63,26 @@ def test_ragged_agrees_with_the_padded_model(model):
         assert float(logits.abs().max()) < 16
         want = torch.log_softmax(logits, -1).gather(1, p[1:, None].cuda())[:, 0]
         assert (s.logprob - want).abs().max() < TOL
+
+
+def test_bad_indices_raise_and_leave_the_generator_usable(model):
+    """What the kernels record is read: pages outside the pool, positions past the
+    RoPE table."""
+    from afd_demo_b200.ops.checks import AFDBoundsError
+
+    prompts = _prompts(model, [20, 70])
+    gen = model.ragged(num_pages=8, page_size=32)
+    want = gen.generate(prompts, 4)
+    table = gen.cache.table
+    gen.cache.table = lambda seqs: table(seqs) + 8
+    with pytest.raises(AFDBoundsError):
+        gen.generate(prompts, 4)
+    gen.cache.table = table
+    assert gen.cache.free_pages == 8
+    most, gen.max_positions = gen.max_positions, 1 << 20
+    with pytest.raises(AFDBoundsError):
+        gen.score(_prompts(model, [most + 1]))
+    gen.max_positions = most
+    for a, b in zip(gen.generate(prompts, 4), want):
+        assert torch.equal(a.tokens, b.tokens)
+    gen.score(prompts)
