@@ -125,6 +125,7 @@ class RaggedGenerator:
 
     # ------------------------------------------------------------- helpers
     def _check_prompts(self, prompts: Sequence[Sequence[int]], new: int) -> List[torch.Tensor]:
+        """The prompts as tensors; `new` positions follow each."""
         if len(prompts) == 0:
             raise ValueError("no prompts")
         got = []
@@ -133,8 +134,8 @@ class RaggedGenerator:
             if t.numel() == 0:
                 raise ValueError(f"prompt {i} is empty")
             if t.numel() + new > self.max_positions:
-                raise ValueError(f"prompt {i}: {t.numel()} tokens and {new} new ones exceed the "
-                                 f"{self.max_positions} positions of the workers")
+                raise ValueError(f"prompt {i}: {t.numel()} tokens and {new} positions after them "
+                                 f"exceed the {self.max_positions} positions of the workers")
             if int(t.min()) < 0 or int(t.max()) >= self.cfg.vocab_size:
                 raise ValueError(f"prompt {i} has a token outside [0, {self.cfg.vocab_size})")
             got.append(t)
@@ -218,7 +219,7 @@ class RaggedGenerator:
             raise ValueError(f"max_new_tokens {max_new_tokens} must be positive")
         if prefill_chunk_size is not None and prefill_chunk_size < 1:
             raise ValueError(f"prefill_chunk_size {prefill_chunk_size} must be positive")
-        ids = self._check_prompts(prompts, max_new_tokens)
+        ids = self._check_prompts(prompts, max_new_tokens - 1)  # the last has no position
         B, dev, page = len(ids), self.device, self.cache.page_size
         seqs: List[int] = []
         try:

@@ -114,3 +114,14 @@ def test_what_a_kernel_recorded_is_raised_once(model, code):
             call()
         assert gen.cache.free_pages == 2
         call()
+
+
+def test_generate_up_to_the_last_position(model):
+    """As the padded path does: the last new token needs no position."""
+    p = _prompts(model, [90])
+    gen = model.ragged(num_pages=6, page_size=16)
+    out = gen.generate(p, 7)
+    assert torch.equal(out[0].tokens, _alone(model, p[0], 7))
+    with pytest.raises(ValueError):
+        gen.generate(p, 8)
+    assert gen.cache.free_pages == 6
