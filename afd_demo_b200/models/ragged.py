@@ -39,8 +39,8 @@ class PagedKVCache:
                  dtype=torch.bfloat16):
         if num_pages < 1:
             raise ValueError(f"num_pages {num_pages} must be positive")
-        if page_size < 16 or page_size % 16:
-            raise ValueError(f"page_size {page_size} must be a multiple of 16")
+        if page_size < 16 or page_size % 16 or page_size > 4096:
+            raise ValueError(f"page_size {page_size} must be a multiple of 16, at most 4096")
         self.page_size = page_size
         self.num_pages = num_pages
         shape = (cfg.num_hidden_layers, num_pages, cfg.num_key_value_heads, page_size,
@@ -273,6 +273,8 @@ class RaggedGenerator:
         """Log-probability of each token of each sequence given the ones before it
         (from the second token on), the entropies, and the most likely tokens. The
         LM head runs on `rows_at_once` positions at a time."""
+        if rows_at_once < 1:
+            raise ValueError(f"rows_at_once {rows_at_once} must be positive")
         ids = self._check_prompts(sequences, 0)
         cfg, dev = self.cfg, self.device
         lens = [p.numel() for p in ids]

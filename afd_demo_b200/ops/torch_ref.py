@@ -216,8 +216,13 @@ def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, D: int) -> None:
     _check(k_pages.dim() == 4 and k_pages.shape == v_pages.shape,
            "k_pages and v_pages must be [pages, kv heads, page_size, head_dim], laid out alike")
     _check(k_pages.shape[3] == D, "q and the pages differ in head_dim")
-    _check(k_pages.shape[2] >= 16 and k_pages.shape[2] % 16 == 0,
+    _check(k_pages.shape[0] >= 1, "the pool has no page")
+    _check(16 <= k_pages.shape[2] <= 4096 and k_pages.shape[2] % 16 == 0,
            "page_size must be a multiple of 16, at most 4096")
+
+
+def _check_scale(scale: Optional[float]) -> None:
+    _check(scale is None or (scale > 0 and math.isfinite(scale)), "scale must be positive")
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
@@ -249,6 +254,7 @@ def qk_norm_rope_paged(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Te
     not stored). Returns q."""
     D, T = q_norm.shape[0], qkv.shape[0]
     _check_pool(k_pages, v_pages, D)
+    _check(k_pages.shape[1] == nkv, "the pages' heads differ from qkv's")
     _check(slots.dtype == torch.int64 and slots.numel() == T,
            "slots must be a contiguous int64 tensor, one per token")
     q, k = qk_norm_rope(qkv, q_norm, k_norm, rope, positions, nq, nkv, eps)
@@ -295,6 +301,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and k.shape[2] == q.shape[2],
            "k and v must be [rows, kv heads, head_dim] with the queries' head_dim")
     _check_heads(q.shape[1], k.shape[1])
+    _check(q.shape[1] // k.shape[1] <= 128, "at most 128 query heads per kv head")
+    _check_scale(scale)
     _check(cu_seqlens_k is not None or k.shape[0] == q.shape[0],
            "k has other rows than q: give cu_seqlens_k")
     cu_k = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
@@ -316,9 +324,18 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
                             page_table: torch.Tensor, seq_lens: torch.Tensor,
                             cu_seqlens: torch.Tensor, scale: Optional[float] = None
                             ) -> torch.Tensor:
+    _check(q.dim() != 3 or k_pages.dim() != 4 or q.shape[1] <= 128 * k_pages.shape[1],
+           "at most 128 query heads per kv head")
+    return _paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, scale)
+
+
+def _paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                     page_table: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float]) -> torch.Tensor:
     _check(q.dim() == 3, "q must be [rows, heads, head_dim]")
     _check_pool(k_pages, v_pages, q.shape[2])
     _check_heads(q.shape[1], k_pages.shape[1])
+    _check_scale(scale)
     n = cu_seqlens.numel() - 1
     for t in (page_table, seq_lens, cu_seqlens):
         _check(t.dtype == torch.int32, "page_table, seq_lens and cu_seqlens must be int32")
@@ -341,7 +358,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                            page_table: torch.Tensor, seq_lens: torch.Tensor,
                            scale: Optional[float] = None) -> torch.Tensor:
     cu = torch.arange(q.shape[0] + 1, dtype=torch.int32)
-    return paged_prefill_attention(q, k_pages, v_pages, page_table, seq_lens, cu, scale)
+    return _paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu, scale)
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0

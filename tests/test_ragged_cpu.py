@@ -157,3 +157,26 @@ def test_query_offsets_are_clamped_and_decreasing_ones_give_zeros(cu, same):
             assert torch.equal(out, call(same))
             assert not out[: same[0]].any() and not out[same[-1]:].any()
             assert out[same[0]: same[-1]].any(-1).all()
+
+
+def test_refusals_are_the_kernels():
+    """What the bindings refuse by value, the CPU statements refuse too."""
+    q, kv = torch.randn(4, 2, 32), torch.randn(4, 1, 32)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            ops.packed_attention(q, kv, kv, _i32([0, 4]), scale=scale)
+    with pytest.raises(ValueError):
+        ops.packed_attention(torch.randn(4, 129, 32), kv, kv, _i32([0, 4]))
+    table, lens = _i32([[0]] * 4), _i32([1] * 4)
+    for pages, kw in ((torch.randn(2, 1, 16, 32), dict(scale=-1.0)), (torch.randn(1, 1, 4112, 32), {}),
+                      (torch.randn(0, 1, 16, 32), {})):
+        with pytest.raises(ValueError):
+            ops.paged_decode_attention(q, pages, pages, table, lens, **kw)
+    wide, pages = torch.randn(4, 129, 32), torch.randn(2, 1, 16, 32)
+    assert ops.paged_decode_attention(wide, pages, pages, table, lens).isfinite().all()
+    with pytest.raises(ValueError):
+        ops.paged_prefill_attention(wide, pages, pages, table, lens, _i32([0, 1, 2, 3, 4]))
+    pages, w = torch.zeros(2, 4, 16, 32), torch.ones(32)
+    with pytest.raises(ValueError):  # one kv head into pages of four
+        ops.qk_norm_rope_paged(torch.randn(4, 4 * 32), w, w, torch.ones(8, 32), pages, pages.clone(),
+                               _i32([0] * 4), torch.arange(4), 2, 1, 1e-6)

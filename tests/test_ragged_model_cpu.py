@@ -125,3 +125,11 @@ def test_generate_up_to_the_last_position(model):
     with pytest.raises(ValueError):
         gen.generate(p, 8)
     assert gen.cache.free_pages == 6
+
+
+def test_more_refusals(model):
+    with pytest.raises(ValueError):
+        model.ragged(num_pages=1, page_size=4112)
+    for rows in (0, -1):
+        with pytest.raises(ValueError):
+            model.ragged(num_pages=1, page_size=16).score([[1, 2]], rows_at_once=rows)
