@@ -341,8 +341,8 @@ __device__ int list_top(Shared<T>& sh, const T* x, int V, int n_blocks, int top_
         k = __reduce_max_sync(0xffffffffu, best);
         unsigned at = 0xffffffffu;
         if (best == k)
-          for (int i = n_blocks - 1; i >= 0; --i)
-            if (i % 32 == lane && sh.keys[i] == k) at = i;
+          for (int i = lane; i < n_blocks; i += 32)
+            if (sh.keys[i] == k) at = min(at, (unsigned)i);
         const int b = (int)__reduce_min_sync(0xffffffffu, at);
         if (lane == 0) sh.sel[r] = b;
         if (b % 32 == lane) sh.keys[b] = 0;
