@@ -98,7 +98,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32 [n + 1], rising). With
     `cu_seqlens_k` the keys have rows of their own and the queries are the last
     positions of their sequence; a query before the first key gives zeros, and so
-    do rows before cu_seqlens[0] and past cu_seqlens[n]. Returns [T, nq * D]."""
+    do rows before cu_seqlens[0] and past cu_seqlens[n]. Returns [T, nq * D].
+
+    The softmax weights are rounded to q's type for their product with v. A NaN or an
+    infinity in v reaches, besides the queries that see it, earlier ones that share a
+    tile with it, up to 63 + 256 nkv / nq positions before it (on CPU any of its
+    sequence): it meets their weights of zero. One in k does not."""
     if not q.is_cuda:
         return torch_ref.packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale)
     return _ext().packed_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale, status)

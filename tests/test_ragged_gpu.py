@@ -327,6 +327,37 @@ def test_packed_attention_neighbours_do_not_mix():
         assert torch.equal(out[:100], want[:100]) and torch.equal(out[160:], want[160:])
 
 
+@pytest.mark.parametrize("nq,nkv,D", [(32, 4, 128), (8, 2, 64), (2, 2, 128)])
+def test_packed_attention_what_nan_reaches(nq, nkv, D):
+    """In k: the queries that see it. In v: those, and at most 63 + 256 nkv / nq
+    positions before them, in its dim alone. Whole keys and split ones."""
+    g = _gen(17)
+    G = nq // nkv
+    for news, total in ((1000, 1000), (16, 5000)):
+        q = _randn(g, news, nq, D)
+        k, v = _randn(g, total, nkv, D), _randn(g, total, nkv, D)
+        cu, cu_k = _cu([news]), _cu([total])
+        want = ops.packed_attention(q, k, v, cu, cu_k).view(news, nkv, G, D)
+        for back in (1, news // 2 + 3, news):
+            at = total - back  # a position that the last `back` queries see
+            first = news - back
+            for bad in (NAN, math.inf):
+                k2, v2 = k.clone(), v.clone()
+                k2[at, 1] = bad
+                v2[at, 1, 7] = bad
+                got = ops.packed_attention(q, k2, v, cu, cu_k).view(news, nkv, G, D)
+                assert torch.equal(got[:, 0], want[:, 0])
+                assert torch.equal(got[:first], want[:first])
+                if bad != bad:
+                    assert got[first:, 1].isnan().all()
+                got = ops.packed_attention(q, k, v2, cu, cu_k).view(news, nkv, G, D)
+                near = max(0, first - 63 - 256 // G)
+                assert torch.equal(got[:near], want[:near])
+                assert not got[first:, 1, :, 7].isfinite().any()
+                got[:, 1, :, 7] = want[:, 1, :, 7]
+                assert torch.equal(got, want)
+
+
 def _leave_nan(rows, width):
     """NaN where the next output of this size will lie."""
     torch.full((rows, width), NAN, device=DEV, dtype=torch.bfloat16)
