@@ -28,7 +28,11 @@
 // The running maximum is raised only when a row's maximum grows by more than 8
 // (in powers of two): P then holds values up to 256, exact in the ratio O / l,
 // and O is rescaled in TMEM only in such steps. P is rounded to the input type
-// for the second product; maxima, sums and both accumulators are fp32.
+// for the second product; maxima, sums and both accumulators are fp32. With P as high
+// part and remainder (as in paged_decode.cu) the second product would run twice, on a
+// tensor pipe that is 57% busy and in the chain that bounds a step; rounded, the error
+// against 64 bits grows from 0.0016, the output's own rounding, to 0.0019..0.0021 in bf16
+// and from 0.00021 to 0.00029 in fp16.
 //
 // TMEM columns: S_A [0,128), S_B [128,256) (two buffers of 64; P over the first
 // 32 of each), O_A [256,256+D), O_B [384,384+D).
@@ -47,7 +51,8 @@
 // over 2000: 24 us, 18.5 with 8).
 //
 // Measured (bf16, 32 heads over 4 of 128): 4 prompts of 2338..8192 tokens, 991
-// GFLOP visible, 865 us, 1.15 PF/s; 32 prompts of 5..1021, 72 us. A step of both row
+// GFLOP visible, 870 us, 1.14 PF/s; 32 prompts of 5..1021, 71 us (short bursts; 900 and
+// 80 in calls repeated for half a second, at lower clocks). A step of both row
 // tiles takes 1820 cycles, for 1024 of products and as many of exponentials (4096
 // tokens: tensor pipe 57%, special function units 61%, issue slots 40%, reads of
 // shared memory by the MMAs 57%): none is full, what is left is the chain of a

@@ -27,8 +27,11 @@
 // tensor pipe has the room, and the output is then rounded once, as the formula is.
 //
 // Split: the 16-key blocks of all (sequence, kv head) items, in order, are cut
-// into equal ranges, one per CTA, whatever the lengths: the last CTA ends when the
-// first does. A CTA joins its 4 warps in shared memory; an item cut by a range
+// into equal ranges, one per CTA, and a range end near an item's end moves there. Over
+// long caches the ranges stay equal (16 sequences of 20000..40960: 399 blocks at most,
+// 392 on average; 150.5 us for 950 MB, 6.3 TB/s). Over short ones moving saves cuts but
+// leaves ranges uneven (32 sequences of 128..4096: 60 blocks at most, 33 on average, 110 and
+// 66 on an SM; 22.5 us, where the bytes take 12.3). A CTA joins its 4 warps in shared memory; an item cut by a range
 // end leaves fp32 partials (O, maximum, sum) in the workspace, and the CTA
 // that counts the last of its parts joins them, in the order of the parts.
 

@@ -13,9 +13,9 @@
 // elements, the next block on its way while one is summed: the block's maximum
 // by one warp reduction (a running maximum of the warp's, so that sums are
 // rescaled only when it moves), then a subtraction, a product, an exponential, an add
-// and a multiply-add per element, in pairs. The loop issues about 100 instructions for a block's 16
-// exponentials a lane, so that the exponentials (a quarter of a warp's lanes a
-// cycle) and not the issue come next after the memory.
+// and a multiply-add per element, in pairs. A block costs about 160 instructions for 16
+// exponentials a lane: 71% of the issue slots and 59% of the special function units
+// are busy (1184 rows, by counter), and issue comes next after the memory.
 //
 // The top tokens cost the pass nothing but the block maxima, which it has
 // anyway and leaves behind: the k blocks with the largest maxima (the earlier
@@ -24,8 +24,11 @@
 // blocks, reads them again (k KB, from L2) and ranks the few elements that reach
 // the smallest of the picked maxima.
 //
-// Measured (4096 rows of 151936, bf16, top 8; 1245 MB): 213 us, 5.8 TB/s. Blocks
-// loaded to registers one ahead took 323, the ring with the maxima in fp32 250.
+// Measured (4096 rows of 151936, bf16, top 8; 1245 MB): 220 us in a burst, 5.7 TB/s, and
+// 247 to 259 in calls repeated for half a second, at lower clocks. Earlier forms, in
+// bursts: blocks loaded to registers one ahead 323, the ring with the maxima in fp32
+// 250; with one multiply-add for an exponent 212, and 216 without a sum of each block (see
+// Running).
 //
 // Few rows are split over several CTAs: each leaves (m, Z, S) and its block
 // maxima in the workspace, and the CTA that counts the row's last part
@@ -196,7 +199,7 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
 // A lane's running sums, all lanes of a warp with the same m. S is kept over
 // ln(2): its terms are e^(x - m) t with the exponent t = (x - m) log2(e). The maximum is
 // subtracted before the scaling. fma(x, log2(e), -m log2(e)) would save one of five
-// packed instructions (4096 rows of bf16 in a loop: 251 us, 254.5 so), but its exponents are
+// packed instructions (4096 rows of bf16: 212 us in a burst, 216 so), but its exponents are
 // all off by the rounding of m log2(e): by 1e-3 at |m| = 3e4, differently for each m that
 // the running maximum took on, and by hundreds at |m| = 1e10.
 template <typename T>
@@ -222,7 +225,8 @@ struct Running {
       b.lift();
       const float2 l2 = make_float2(kLog2e, kLog2e), nm = make_float2(-m, -m);
       // The block by itself first: a long row's sums then meet 8 times fewer
-      // roundings, which for equal logits all go the same way.
+      // roundings, which for equal logits all go the same way (262656 sorted logits are
+      // 1.1e-6 off without; 4096 rows of 151936 take 216 us without, 220 so).
       float2 zb, sb;
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
