@@ -113,8 +113,9 @@ void check_ints(const at::Tensor& t, const at::Tensor& like, int64_t n, const ch
 
 int* status_ptr(const OptTensor& s, const at::Tensor& like) {
   if (!s.has_value() || !s->defined()) return nullptr;
-  TORCH_CHECK_VALUE(s->device() == like.device() && s->scalar_type() == at::kInt && s->numel() >= 2,
-              "status must be an int32 tensor of 2 on the same device");
+  TORCH_CHECK_VALUE(s->device() == like.device() && s->scalar_type() == at::kInt &&
+                        s->numel() >= 2 && s->is_contiguous(),
+                    "status must be a contiguous int32 tensor of 2 on the same device");
   return s->data_ptr<int>();
 }
 

@@ -847,3 +847,18 @@ def test_page_tables_past_the_positions_of_an_int_are_refused():
             else:
                 with pytest.raises(ValueError):
                     call(table)
+
+
+def test_status_of_other_layouts_is_refused():
+    """The kernels write two neighbouring words."""
+    g = _gen(18)
+    q, pages = _randn(g, 2, 4, 64), _randn(g, 2, 4, 16, 64)
+    one, three = _i32([0]), _i32([0, 0, 0])
+    for bad in (one, one.expand(2), three[::2], three.long(), three.cpu()):
+        for call in (lambda s: ops.paged_decode_attention(q, pages, pages, _i32([[0], [1]]),
+                                                          _i32([3, 99]), status=s),
+                     lambda s: ops.packed_attention(q, q, q, _i32([0, 2]), status=s)):
+            with pytest.raises(ValueError):
+                call(bad)
+    ops.paged_decode_attention(q, pages, pages, _i32([[0], [1]]), _i32([3, 99]), status=three)
+    assert three.tolist()[0] == 3 and three.tolist()[2] == 0
