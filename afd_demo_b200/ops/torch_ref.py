@@ -222,7 +222,8 @@ def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, D: int) -> None:
 
 
 def _check_scale(scale: Optional[float]) -> None:
-    _check(scale is None or (scale > 0 and math.isfinite(scale)), "scale must be positive")
+    s = 1.0 if scale is None else float(torch.tensor(scale, dtype=torch.float32))
+    _check(s > 0 and math.isfinite(s), "scale must be positive, in 32 bits")
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,

@@ -145,8 +145,8 @@ void take_pool(Args& a, const at::Tensor& k_pages, const at::Tensor& v_pages,
 }
 
 float scale_of(c10::optional<double> scale, int D) {
-  TORCH_CHECK_VALUE(!scale.has_value() || (*scale > 0 && std::isfinite(*scale)),
-                    "scale must be positive");
+  TORCH_CHECK_VALUE(!scale.has_value() || ((float)*scale > 0 && std::isfinite((float)*scale)),
+                    "scale must be positive, in 32 bits");
   return scale.has_value() ? (float)*scale : 1.f / std::sqrt((float)D);
 }
 

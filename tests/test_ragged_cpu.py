@@ -180,3 +180,10 @@ def test_refusals_are_the_kernels():
     with pytest.raises(ValueError):  # one kv head into pages of four
         ops.qk_norm_rope_paged(torch.randn(4, 4 * 32), w, w, torch.ones(8, 32), pages, pages.clone(),
                                _i32([0] * 4), torch.arange(4), 2, 1, 1e-6)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e39])
+def test_scales_that_are_no_float_are_refused(scale):
+    q = torch.randn(4, 2, 32)
+    with pytest.raises(ValueError):
+        ops.packed_attention(q, q, q, _i32([0, 4]), scale=scale)

@@ -862,3 +862,15 @@ def test_status_of_other_layouts_is_refused():
                 call(bad)
     ops.paged_decode_attention(q, pages, pages, _i32([[0], [1]]), _i32([3, 99]), status=three)
     assert three.tolist()[0] == 3 and three.tolist()[2] == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, NAN, math.inf, 1e-50, 1e39])
+def test_scales_that_are_no_positive_float_are_refused(scale):
+    g = _gen(19)
+    q, pages, table, lens = _randn(g, 2, 4, 64), _randn(g, 2, 4, 16, 64), _i32([[0]] * 2), _i32([3, 4])
+    for call in (lambda: ops.paged_decode_attention(q, pages, pages, table, lens, scale=scale),
+                 lambda: ops.packed_attention(q, q, q, _i32([0, 2]), scale=scale),
+                 lambda: ops.paged_prefill_attention(q, pages, pages, table, lens, _i32([0, 1, 2]),
+                                                     scale=scale)):
+        with pytest.raises(ValueError):
+            call()
