@@ -27,7 +27,11 @@
 //
 // The running maximum is raised only when a row's maximum grows by more than 8
 // (in powers of two): P then holds values up to 256, exact in the ratio O / l,
-// and O is rescaled in TMEM only in such steps. P is rounded to the input type
+// and O is rescaled in TMEM only in such steps. The exponents are fma(s, c, -m) with
+// c = scale log2(e) and m = c max(s) rounded: every weight of a row has the same factor
+// for that rounding. Where it could leave the range (|m| from 2^26 on, scores that only
+// an overflow makes) it is taken out again, see Ref; without that the 32 prompts below
+// take 71.3 us, 72.6 so, and the 4 long ones 876, 882. P is rounded to the input type
 // for the second product; maxima, sums and both accumulators are fp32. With P as high
 // part and remainder (as in paged_decode.cu) the second product would run twice, on a
 // tensor pipe that is 57% busy and in the chain that bounds a step; rounded, the error
@@ -51,8 +55,8 @@
 // over 2000: 24 us, 18.5 with 8).
 //
 // Measured (bf16, 32 heads over 4 of 128): 4 prompts of 2338..8192 tokens, 991
-// GFLOP visible, 870 us, 1.14 PF/s; 32 prompts of 5..1021, 71 us (short bursts; 900 and
-// 80 in calls repeated for half a second, at lower clocks). A step of both row
+// GFLOP visible, 882 us, 1.12 PF/s; 32 prompts of 5..1021, 73 us (short bursts; 910 and
+// 81 in calls repeated for half a second, at lower clocks). A step of both row
 // tiles takes 1820 cycles, for 1024 of products and as many of exponentials (4096
 // tokens: tensor pipe 57%, special function units 61%, issue slots 40%, reads of
 // shared memory by the MMAs 57%): none is full, what is left is the chain of a
@@ -79,6 +83,20 @@ constexpr int kThreads = 320;
 // Parts of an item's keys: at most kMaxParts, of kMinPart steps at least.
 constexpr int kMaxParts = 32;
 constexpr int kMinPart = 8;
+
+// What a row's weights are relative to: 2^(m + r), m = c s rounded for its largest score s
+// and r the rounding where |m| is large (up to 2 left in below that), else 0.
+struct Ref {
+  float m, r;
+};
+constexpr float kFar = 67108864.f;  // 2^26
+
+__device__ __forceinline__ Ref ref_of(float s, float c) {
+  const float m = s * c;
+  return {m, fabsf(m) >= kFar && fabsf(m) < INFINITY ? fmaf(s, c, -m) : 0.f};
+}
+// Exponent of a / b, -inf where a has seen no key.
+__device__ __forceinline__ float over(const Ref& a, const Ref& b) { return (a.m - b.m) + (a.r - b.r); }
 
 struct Item {
   int steps;    // 64-key steps of this part; 0: no key; -1: no more work
@@ -539,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = (uint32_t)(qq * 32) << 16;
     const uint32_t t_o = tmem + 256 + x * 128 + lane_off;
     const float scale_log2 = a.scale * 1.4426950408889634f;
+    const float growth = fminf(8.f / scale_log2, 1e38f);
     int g = 0, taken = 0;
     bool ok = true;
     // TMEM accesses are warp-collective: every branch around them is
@@ -561,7 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = w.pos0 + w.tokens;
       const int pos = min(w.pos0 + tok, len - 1);
       const int warp_pos0 = min(w.pos0 + tok_first, len - 1);
-      float m = -INFINITY;
+      float top = -INFINITY;  // the running maximum, a score
+      bool far = false;       // a row of the warp has a remainder in its Ref
       float2 l2 = make_float2(0.f, 0.f);
       for (int i = 0; i < w.steps; ++i, ++g) {
         const int buf = g & 1, key0 = i * kKeys;
@@ -599,15 +619,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[k + 2 * e], s[k + 2 * e + 1]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[kKeys - 4 + e]);
-        const float rmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale_log2;
-        const bool grow = rmax > m + 8.f;
+        const float rmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+        const bool grow = rmax > top + growth;
         if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? rmax : m;
+          const float top_new = grow ? rmax : top;
+          const Ref now = ref_of(top_new, scale_log2);
           if (i > 0) {
             // O holds steps 0 .. i-1 once P(i-1) V is done
             if (!wait_all(&pv_done[2 * x + (buf ^ 1)], ((g - 1) >> 1) & 1, 253)) break;
             tc_fence_after();
-            const float alpha = grow ? exp2_approx(m - m_new) : 1.f;
+            const float alpha = grow ? exp2_approx(over(ref_of(top, scale_log2), now)) : 1.f;
             l2.x *= alpha;
             l2.y *= alpha;
 #pragma unroll
@@ -619,12 +640,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st16(t_o + c * 16, o);
             }
           }
-          m = m_new;
+          top = top_new;
+          far = __any_sync(0xffffffffu, now.r != 0.f);
         }
-        // p = 2^(s scale log2(e) - m); a masked s = -inf gives 0, also in a row
-        // that has seen no key yet (m = -inf)
-        const float neg_m = m == -INFINITY ? 0.f : -m;
-        const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(neg_m, neg_m);
+        // p = 2^(s c - m); a masked s = -inf gives 0, also in a row that has seen
+        // no key yet (m = -inf)
+        float factor = scale_log2, neg_m = top == -INFINITY ? 0.f : -(top * scale_log2);
+        if (far) {
+          const float r = ref_of(top, scale_log2).r;
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k) s[k] = fmaf(s[k], factor, neg_m) - r;
+          factor = 1.f;
+          neg_m = 0.f;
+        }
+        const float2 sc2 = make_float2(factor, factor), nm2 = make_float2(neg_m, neg_m);
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
           uint32_t pk[16];
@@ -653,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (a.splits > 1 && has_token && tok < w.tokens) {
         const size_t r = (size_t)(w.row0 + tok) * a.nq + w.kvh * G + row % G;
         if (w.parts < 256) a.n_parts[r] = w.parts;
-        a.part_ml[(size_t)(w.parts >> 8) * a.T * a.nq + r] = make_float2(m, l);
+        a.part_ml[(size_t)(w.parts >> 8) * a.T * a.nq + r] = make_float2(top, l);
       }
       // Through shared memory, so that a store instruction covers whole 128-byte
       // lines of four rows (a row a lane took 4100 cycles for an item's rows).
@@ -720,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the rows that have several, D / 4 threads a row:
-//   out = sum_p w_p O_p / sum_p w_p l_p,  w_p = 2^(m_p - max m)
+//   out = sum_p w_p O_p / sum_p w_p l_p,  w_p = Ref of the part / Ref of the largest
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_parts_kernel(PackedAttnArgs a) {
   constexpr int kLanes = D / 4;
@@ -733,6 +762,8 @@ __global__ void __launch_bounds__(128) join_parts_kernel(PackedAttnArgs a) {
   if (parts <= 1) return;
   float most = -INFINITY;
   for (int p = 0; p < parts; ++p) most = fmaxf(most, a.part_ml[p * rows + r].x);
+  const float scale_log2 = a.scale * 1.4426950408889634f;
+  const Ref ref = ref_of(most, scale_log2);
   const int at = threadIdx.x % kLanes * 4;
   float l = 0.f, o[4] = {};
 #pragma unroll 4
@@ -740,7 +771,7 @@ __global__ void __launch_bounds__(128) join_parts_kernel(PackedAttnArgs a) {
     const float2 ml = a.part_ml[p * rows + r];
     const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * rows + r) * D + at);
     if (ml.y == 0.f) continue;  // the row saw none of the part's keys
-    const float w = exp2_approx(ml.x - most);
+    const float w = exp2_approx(over(ref_of(ml.x, scale_log2), ref));
     l = fmaf(w, ml.y, l);
     o[0] = fmaf(w, v.x, o[0]);
     o[1] = fmaf(w, v.y, o[1]);

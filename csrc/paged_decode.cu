@@ -440,8 +440,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float x[4];
+        // rounded here, not within a multiply-add, so that the largest one's x - m is 0
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = s[n][e] * scale_log2;
+        for (int e = 0; e < 4; ++e) x[e] = __fmul_rn(s[n][e], scale_log2);
         // the maximum moves only when it grows by more than 8 (powers of two)
         const bool grow = fmaxf(x[0], x[2]) > m[n][0] + 8.f || fmaxf(x[1], x[3]) > m[n][1] + 8.f;
         if (__any_sync(0xffffffffu, grow)) {

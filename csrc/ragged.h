@@ -81,7 +81,7 @@ struct PackedAttnArgs {
   int* counter;             // [1], zero; left zero
   int splits;               // parts of a block's keys at most; 1: none is split
   float* part_o;            // filled in by the launch: O [splits, T, nq, D],
-  float2* part_ml;          // maximum and sum [splits, T, nq],
+  float2* part_ml;          // largest score and sum [splits, T, nq],
   int* n_parts;             // parts [T, nq]
 };
 // Parts that fill the GPU where there are few blocks, for keys up to most_keys.

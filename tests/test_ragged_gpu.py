@@ -174,6 +174,32 @@ def test_paged_decode_nan_is_kept(nq, nkv, D, lens):
             check(ops.paged_decode_attention(q, k2, vp, table, seq), b, list(range(G, 2 * G)))
 
 
+@pytest.mark.parametrize("dtype,power", [(t, p) for t in DTYPES for p in (0, 8, 16, 24)] +
+                         [(torch.bfloat16, p) for p in (32, 48, 90)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("n,total", [(40, 700), (8, 5000)])
+def test_attention_of_huge_scores(dtype, power, sign, n, total):
+    """Finite scores of any size, exact in fp32: 2^power times a whole number of 13 at
+    most (13 scale log2(e) is no float). From 2^8 on the keys with the largest share the
+    weight and the others have none (2^-30 of it at most)."""
+    g = _gen(20)
+    nq, nkv, D, pages, a = 4, 2, 64, -(-total // 64), power // 2
+    q = torch.zeros(n, nq, D, device=DEV, dtype=dtype)
+    q[..., 3] = 2.0 ** a
+    k, v = torch.zeros(total, nkv, D, device=DEV, dtype=dtype), _randn(g, total, nkv, D, dtype=dtype)
+    k[..., 3] = (sign * torch.randint(0, 14, (total, nkv), generator=g, device=DEV)
+                 * 2.0 ** (power - a)).to(dtype)
+    kp, vp = (torch.cat([x, x[:64 * pages - total]]).view(pages, 64, nkv, D).transpose(1, 2)
+              .contiguous() for x in (k, v))
+    table = torch.arange(pages, device=DEV, dtype=torch.int32)[None]
+    exact = _exact_rows(q, k, v)
+    for out in (ops.packed_attention(q, k, v, _cu([n]), _cu([total])),
+                ops.paged_prefill_attention(q, kp, vp, table, _i32([total]), _cu([n]))):
+        _close(out, exact, dtype)
+    _close(ops.paged_decode_attention(q[-1:], kp, vp, table, _i32([total])),
+           tuple(x[-1:] for x in exact), dtype)
+
+
 def test_paged_decode_strides():
     """q as a view of a projection; the pool as a layer of a larger buffer, with
     k and v interleaved page by page; a table wider than its view."""
