@@ -33,10 +33,10 @@
 // an overflow makes) it is taken out again, see Ref; without that the 32 prompts below
 // take 71.3 us, 72.6 so, and the 4 long ones 876, 882. P is rounded to the input type
 // for the second product; maxima, sums and both accumulators are fp32. With P as high
-// part and remainder (as in paged_decode.cu) the second product would run twice, on a
-// tensor pipe that is 57% busy and in the chain that bounds a step; rounded, the error
-// against 64 bits grows from 0.0016, the output's own rounding, to 0.0019..0.0021 in bf16
-// and from 0.00021 to 0.00029 in fp16.
+// part and remainder, as in paged_decode.cu, the second product runs twice in the chain
+// that bounds a step: 32 prompts 92 us, 4 long ones 1220 (73 and 884 rounded, next
+// below). The error against 64 bits is then the output's own rounding, 0.0016 in bf16 and
+// 0.00021 in fp16; rounded it is 0.0019..0.0022 and 0.00029.
 //
 // TMEM columns: S_A [0,128), S_B [128,256) (two buffers of 64; P over the first
 // 32 of each), O_A [256,256+D), O_B [384,384+D).
@@ -55,7 +55,7 @@
 // over 2000: 24 us, 18.5 with 8).
 //
 // Measured (bf16, 32 heads over 4 of 128): 4 prompts of 2338..8192 tokens, 991
-// GFLOP visible, 882 us, 1.12 PF/s; 32 prompts of 5..1021, 73 us (short bursts; 910 and
+// GFLOP visible, 884 us, 1.12 PF/s; 32 prompts of 5..1021, 73 us (short bursts; 913 and
 // 81 in calls repeated for half a second, at lower clocks). A step of both row
 // tiles takes 1820 cycles, for 1024 of products and as many of exponentials (4096
 // tokens: tensor pipe 57%, special function units 61%, issue slots 40%, reads of
