@@ -34,9 +34,9 @@
 // take 71.3 us, 72.6 so, and the 4 long ones 876, 882. P is rounded to the input type
 // for the second product; maxima, sums and both accumulators are fp32. With P as high
 // part and remainder, as in paged_decode.cu, the second product runs twice in the chain
-// that bounds a step: 32 prompts 92 us, 4 long ones 1220 (73 and 884 rounded, next
-// below). The error against 64 bits is then the output's own rounding, 0.0016 in bf16 and
-// 0.00021 in fp16; rounded it is 0.0019..0.0022 and 0.00029.
+// that bounds a step: 32 prompts 92 us, 4 long ones 1220 (73 and 884 with P rounded).
+// The error against 64 bits is then the output's own rounding, 0.0016 in bf16 and 0.00021
+// in fp16; with P rounded it is 0.0019..0.0022 and 0.00029.
 //
 // TMEM columns: S_A [0,128), S_B [128,256) (two buffers of 64; P over the first
 // 32 of each), O_A [256,256+D), O_B [384,384+D).
